@@ -540,4 +540,59 @@ hipError_t launch_advance(int* pos, const int* active, int rows, hipStream_t s,
                           const uint32_t* tok = nullptr, uint32_t* hist = nullptr,
                           long hist_stride = 0);
 
+// ---------------------------------------------------------------------------
+// 8-bit caches (q8_kernels.hip) and drafted tokens (verify_kernels.hip)
+// ---------------------------------------------------------------------------
+
+// akh_q8_cache with its buffer's parts.
+struct Q8Cache {
+  int8_t* k;   // codes [slots][kv_heads][cap][row]
+  int8_t* v;
+  int8_t* ke;  // exponents [slots][kv_heads][cap]
+  int8_t* ve;
+  uint32_t slots, max_rows, cap, row, kv_heads, head_dim;
+};
+// A launch's grid holds at most this many blocks.
+constexpr uint64_t kMaxBlocks = 0x7FFFFFFF;
+hipError_t launch_cache_write_q8(const float* k, const float* v, const Q8Cache& c, uint32_t batch,
+                                 uint32_t rows, uint32_t stride, const uint32_t* pos,
+                                 const uint32_t* counts, hipStream_t s);
+hipError_t launch_cache_read_q8(const Q8Cache& c, float* k, float* v, uint32_t batch,
+                                uint32_t rows, uint32_t stride, const uint32_t* pos,
+                                const uint32_t* counts, hipStream_t s);
+
+struct AttnQ8Args {
+  const float* q;
+  float* out;
+  float* lse;  // or null
+  Q8Cache c;
+  Q8Cache pre;                 // with prefix_len
+  const uint32_t* prefix_len;  // null: no prefix
+  const uint32_t* pos;
+  const uint32_t* counts;  // or null
+  uint32_t batch, rows, heads, q_stride, out_stride, max_len;
+  float scale;
+  void* ws;
+  int num_cus;
+};
+size_t attn_q8_workspace_bytes(const AttnQ8Args& a);
+hipError_t launch_attn_q8(const AttnQ8Args& a, hipStream_t s);
+
+struct VerifyArgs {
+  const float* target;     // [batch, rows + 1, n]
+  const float* draft;      // [batch, rows, n] or null
+  const uint32_t* tokens;  // [batch, rows]
+  const uint32_t* counts;  // or null
+  const double* uniforms;  // [batch, rows + 1]
+  uint32_t* out_tokens;    // [batch, rows + 1]
+  uint32_t* out_counts;    // [batch]
+  float* chance;           // [batch, rows] or null
+  uint32_t batch, rows, n;
+  float temperature;
+  void* ws;
+};
+size_t verify_workspace_bytes(uint32_t batch, uint32_t rows, uint32_t n);
+uint64_t verify_blocks(uint32_t batch, uint32_t rows, uint32_t n);
+hipError_t launch_verify(const VerifyArgs& a, hipStream_t s);
+
 }  // namespace akh

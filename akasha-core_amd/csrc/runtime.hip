@@ -660,6 +660,242 @@ akh_status sample_rows_into(akh_backend* be, const float* logits, uint32_t rows,
 }  // namespace
 
 // ---------------------------------------------------------------------------
+// 8-bit caches, attention over them, drafted tokens
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// Makes the backend's device current for a launch and puts the caller's back.
+struct DeviceScope {
+  int was = -1;
+  hipError_t err;
+  explicit DeviceScope(int device) {
+    err = hipGetDevice(&was);
+    if (err == hipSuccess && was != device) {
+      err = hipSetDevice(device);
+    } else {
+      was = -1;
+    }
+  }
+  ~DeviceScope() {
+    if (was >= 0) (void)hipSetDevice(was);
+  }
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The parts of a cache's buffer, and its size.
+akh_status q8_parts(const akh_q8_cache& c, Q8Cache* out, size_t* bytes) {
+  CHECK_ARG(c.head_dim >= 1 && c.head_dim <= 128, "q8 cache: head_dim must be 1..128");
+  CHECK_ARG(c.slots && c.kv_heads && c.max_rows, "q8 cache: empty shape");
+  CHECK_ARG(c.max_rows <= (1u << 30), "q8 cache: max_rows exceeds 2^30");
+  out->slots = c.slots;
+  out->max_rows = c.max_rows;
+  out->kv_heads = c.kv_heads;
+  out->head_dim = c.head_dim;
+  out->cap = (c.max_rows + 31) / 32 * 32;
+  out->row = c.head_dim <= 64 ? 64 : 128;
+  const unsigned __int128 heads = (unsigned __int128)c.slots * c.kv_heads * out->cap;
+  CHECK_ARG(heads * 2 * (out->row + 1) <= ((size_t)1 << 46), "q8 cache: over 2^46 bytes");
+  const size_t rows = (size_t)heads;
+  out->k = static_cast<int8_t*>(c.data);
+  out->v = out->k + rows * out->row;
+  out->ke = out->v + rows * out->row;
+  out->ve = out->ke + rows;
+  if (bytes) *bytes = rows * 2 * (out->row + 1);
+  return AKH_OK;
+}
+
+// Checks of a cache_write / cache_read call.
+akh_status q8_rows_args(const akh_q8_cache& cache, uint32_t batch, uint32_t rows, uint32_t stride,
+                        const uint32_t* pos, Q8Cache* c) {
+  akh_status st = q8_parts(cache, c, nullptr);
+  if (st != AKH_OK) return st;
+  CHECK_ARG(cache.data && aligned16(cache.data),
+            "q8 cache: the buffer must be set and aligned to 16 bytes");
+  CHECK_ARG(pos, "q8 cache rows: pos is NULL");
+  CHECK_ARG(batch <= c->slots, "q8 cache rows: batch exceeds the cache's slots");
+  CHECK_ARG((uint64_t)stride >= (uint64_t)c->kv_heads * c->head_dim,
+            "q8 cache rows: row stride below kv_heads * head_dim");
+  CHECK_ARG((unsigned __int128)batch * rows * 2 * c->kv_heads <= kMaxBlocks,
+            "q8 cache rows: too many rows for one call");
+  return AKH_OK;
+}
+
+// Checks of an attention call's sizes, as kernel arguments.
+akh_status attn_q8_args(const akh_attn_q8& s, const akh_q8_cache& cache,
+                        const akh_q8_cache* prefix, int num_cus, AttnQ8Args* a) {
+  akh_status st = q8_parts(cache, &a->c, nullptr);
+  if (st == AKH_OK && prefix) st = q8_parts(*prefix, &a->pre, nullptr);
+  if (st != AKH_OK) return st;
+  CHECK_ARG(!prefix || (a->pre.kv_heads == a->c.kv_heads && a->pre.head_dim == a->c.head_dim),
+            "q8 attention: the prefix's kv_heads and head_dim must be the cache's");
+  CHECK_ARG(s.heads && s.heads % a->c.kv_heads == 0,
+            "q8 attention: heads must be a multiple of kv_heads");
+  CHECK_ARG(s.batch <= a->c.slots, "q8 attention: batch exceeds the cache's slots");
+  const uint64_t width = (uint64_t)s.heads * a->c.head_dim;
+  CHECK_ARG(s.q_stride >= width && s.out_stride >= width,
+            "q8 attention: row stride below heads * head_dim");
+  CHECK_ARG(isfinite(s.scale), "q8 attention: scale must be finite");
+  CHECK_ARG((unsigned __int128)s.batch * s.rows * s.heads <= (1u << 24),
+            "q8 attention: batch * rows * heads exceeds 2^24");
+  a->batch = s.batch;
+  a->rows = s.rows;
+  a->heads = s.heads;
+  a->q_stride = s.q_stride;
+  a->out_stride = s.out_stride;
+  a->scale = s.scale;
+  a->max_len = s.max_len && s.max_len < a->c.max_rows ? s.max_len : a->c.max_rows;
+  a->num_cus = num_cus;
+  return AKH_OK;
+}
+
+akh_status attn_q8(akh_backend* be, const float* q, const akh_q8_cache* prefix,
+                   const uint32_t* prefix_len, const akh_q8_cache& cache, float* out, float* lse,
+                   const akh_attn_q8& shape, const uint32_t* pos, const uint32_t* counts,
+                   void* workspace, size_t workspace_bytes) {
+  AttnQ8Args a{};
+  akh_status st = attn_q8_args(shape, cache, prefix, be->num_cus, &a);
+  if (st != AKH_OK) return st;
+  CHECK_ARG(q && out && pos, "q8 attention: NULL buffer");
+  CHECK_ARG(cache.data && aligned16(cache.data) &&
+                (!prefix || (prefix->data && aligned16(prefix->data))),
+            "q8 attention: the caches' buffers must be set and aligned to 16 bytes");
+  if (!shape.batch || !shape.rows) return AKH_OK;
+  a.q = q;
+  a.out = out;
+  a.lse = lse;
+  a.prefix_len = prefix ? prefix_len : nullptr;
+  a.pos = pos;
+  a.counts = counts;
+  a.ws = workspace;
+  const size_t need = attn_q8_workspace_bytes(a);
+  CHECK_ARG(!need || (workspace && aligned16(workspace) && workspace_bytes >= need),
+            "q8 attention: workspace missing, unaligned or smaller than akh_attn_q8_workspace");
+  DeviceScope scope(be->device);
+  HIP_TRY(scope.err);
+  HIP_TRY(launch_attn_q8(a, be->stream));
+  return AKH_OK;
+}
+
+}  // namespace
+
+extern "C" akh_status akh_q8_cache_bytes(const akh_q8_cache* cache, size_t* bytes) {
+  CHECK_ARG(cache && bytes, "akh_q8_cache_bytes: NULL argument");
+  Q8Cache c;
+  return q8_parts(*cache, &c, bytes);
+}
+
+extern "C" akh_status akh_cache_write_q8(akh_backend* be, const float* k, const float* v,
+                                         akh_q8_cache cache, uint32_t batch, uint32_t rows,
+                                         uint32_t src_stride, const uint32_t* pos,
+                                         const uint32_t* counts) {
+  BE_CHECK(be);
+  Q8Cache c;
+  akh_status st = q8_rows_args(cache, batch, rows, src_stride, pos, &c);
+  if (st != AKH_OK) return st;
+  CHECK_ARG(k && v, "akh_cache_write_q8: NULL buffer");
+  if (!batch || !rows) return AKH_OK;
+  DeviceScope scope(be->device);
+  HIP_TRY(scope.err);
+  HIP_TRY(launch_cache_write_q8(k, v, c, batch, rows, src_stride, pos, counts, be->stream));
+  return AKH_OK;
+}
+
+extern "C" akh_status akh_cache_read_q8(akh_backend* be, akh_q8_cache cache, float* k, float* v,
+                                        uint32_t batch, uint32_t rows, uint32_t dst_stride,
+                                        const uint32_t* pos, const uint32_t* counts) {
+  BE_CHECK(be);
+  Q8Cache c;
+  akh_status st = q8_rows_args(cache, batch, rows, dst_stride, pos, &c);
+  if (st != AKH_OK) return st;
+  if (!batch || !rows || (!k && !v)) return AKH_OK;
+  DeviceScope scope(be->device);
+  HIP_TRY(scope.err);
+  HIP_TRY(launch_cache_read_q8(c, k, v, batch, rows, dst_stride, pos, counts, be->stream));
+  return AKH_OK;
+}
+
+extern "C" akh_status akh_attn_q8_workspace(const akh_attn_q8* shape, const akh_q8_cache* cache,
+                                            const akh_q8_cache* prefix, size_t* bytes) {
+  CHECK_ARG(shape && cache && bytes, "akh_attn_q8_workspace: NULL argument");
+  AttnQ8Args a{};
+  akh_status st = attn_q8_args(*shape, *cache, prefix, 256, &a);
+  if (st != AKH_OK) return st;
+  *bytes = attn_q8_workspace_bytes(a);
+  return AKH_OK;
+}
+
+extern "C" akh_status akh_attn_cached_q8(akh_backend* be, const float* q, akh_q8_cache cache,
+                                         float* out, float* lse, akh_attn_q8 shape,
+                                         const uint32_t* pos, const uint32_t* counts,
+                                         void* workspace, size_t workspace_bytes) {
+  BE_CHECK(be);
+  return attn_q8(be, q, nullptr, nullptr, cache, out, lse, shape, pos, counts, workspace,
+                 workspace_bytes);
+}
+
+extern "C" akh_status akh_attn_prefix_q8(akh_backend* be, const float* q, akh_q8_cache prefix,
+                                         const uint32_t* prefix_len, akh_q8_cache cache,
+                                         float* out, float* lse, akh_attn_q8 shape,
+                                         const uint32_t* pos, const uint32_t* counts,
+                                         void* workspace, size_t workspace_bytes) {
+  BE_CHECK(be);
+  CHECK_ARG(prefix_len, "akh_attn_prefix_q8: prefix_len is NULL");
+  return attn_q8(be, q, &prefix, prefix_len, cache, out, lse, shape, pos, counts, workspace,
+                 workspace_bytes);
+}
+
+extern "C" akh_status akh_verify_drafts_workspace(uint32_t batch, uint32_t rows, uint32_t n,
+                                                  size_t* bytes) {
+  CHECK_ARG(bytes, "akh_verify_drafts_workspace: bytes is NULL");
+  CHECK_ARG(n > 0 && n <= (uint32_t)kMaxSampleVocab, "akh_verify_drafts: n must be 1..2^20");
+  CHECK_ARG(rows <= 1024 && batch <= (1u << 20), "akh_verify_drafts: rows above 1024 or batch above 2^20");
+  CHECK_ARG(verify_blocks(batch, rows, n) <= kMaxBlocks, "akh_verify_drafts: too many rows for one call");
+  *bytes = verify_workspace_bytes(batch, rows, n);
+  return AKH_OK;
+}
+
+extern "C" akh_status akh_verify_drafts(akh_backend* be, const float* target, const float* draft,
+                                        const uint32_t* tokens, uint32_t batch, uint32_t rows,
+                                        uint32_t n, float temperature, const uint32_t* counts,
+                                        const double* uniforms, uint32_t* out_tokens,
+                                        uint32_t* out_counts, float* chance, void* workspace,
+                                        size_t workspace_bytes) {
+  BE_CHECK(be);
+  size_t need = 0;
+  akh_status st = akh_verify_drafts_workspace(batch, rows, n, &need);
+  if (st != AKH_OK) return st;
+  CHECK_ARG(target && out_tokens && out_counts && (tokens || !rows),
+            "akh_verify_drafts: NULL buffer");
+  CHECK_ARG(!isnan(temperature), "akh_verify_drafts: temperature is NaN");
+  CHECK_ARG(temperature <= 0.0f || uniforms,
+            "akh_verify_drafts: sampling (temperature > 0) needs uniforms");
+  CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= need,
+            "akh_verify_drafts: workspace missing, unaligned or smaller than "
+            "akh_verify_drafts_workspace");
+  if (!batch) return AKH_OK;
+  VerifyArgs a{};
+  a.target = target;
+  a.draft = temperature > 0.0f ? draft : nullptr;
+  a.tokens = tokens;
+  a.counts = counts;
+  a.uniforms = uniforms;
+  a.out_tokens = out_tokens;
+  a.out_counts = out_counts;
+  a.chance = chance;
+  a.batch = batch;
+  a.rows = rows;
+  a.n = n;
+  a.temperature = temperature;
+  a.ws = workspace;
+  DeviceScope scope(be->device);
+  HIP_TRY(scope.err);
+  HIP_TRY(launch_verify(a, be->stream));
+  return AKH_OK;
+}
+
+// ---------------------------------------------------------------------------
 // Model weights
 // ---------------------------------------------------------------------------
 

@@ -85,6 +85,22 @@ class Sampling(C.Structure):
                 ("repetition_penalty", C.c_float)]
 
 
+class Q8CacheC(C.Structure):
+    """akh_q8_cache: an 8-bit cache's buffer and shape."""
+
+    _fields_ = [("data", C.c_void_p), ("slots", C.c_uint32), ("max_rows", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class AttnQ8(C.Structure):
+    """akh_attn_q8: an attention call's sizes (strides in floats; max_len 0:
+    the cache's max_rows)."""
+
+    _fields_ = [("batch", C.c_uint32), ("rows", C.c_uint32), ("heads", C.c_uint32),
+                ("q_stride", C.c_uint32), ("out_stride", C.c_uint32), ("scale", C.c_float),
+                ("max_len", C.c_uint32)]
+
+
 class CheckpointInfo(C.Structure):
     """akh_checkpoint_info_t: V3Body's header (src/nn/checkpoint.rs:20-35)."""
 
@@ -201,6 +217,16 @@ _SIGS = {
     "akh_argmax_rows": (ST, [P, P, U32, U32, P]),
     "akh_sample_rows": (ST, [P, P, U32, U32, Sampling, P, U32, P, P, P]),
     "akh_sample_rows_noalloc": (ST, [P, P, U32, U32, Sampling, P, U32, P, P, P]),
+    "akh_q8_cache_bytes": (ST, [C.POINTER(Q8CacheC), C.POINTER(C.c_size_t)]),
+    "akh_cache_write_q8": (ST, [P, P, P, Q8CacheC, U32, U32, U32, P, P]),
+    "akh_cache_read_q8": (ST, [P, Q8CacheC, P, P, U32, U32, U32, P, P]),
+    "akh_attn_q8_workspace": (ST, [C.POINTER(AttnQ8), C.POINTER(Q8CacheC), C.POINTER(Q8CacheC),
+                                   C.POINTER(C.c_size_t)]),
+    "akh_attn_cached_q8": (ST, [P, P, Q8CacheC, P, P, AttnQ8, P, P, P, C.c_size_t]),
+    "akh_attn_prefix_q8": (ST, [P, P, Q8CacheC, P, Q8CacheC, P, P, AttnQ8, P, P, P, C.c_size_t]),
+    "akh_verify_drafts_workspace": (ST, [U32, U32, U32, C.POINTER(C.c_size_t)]),
+    "akh_verify_drafts": (ST, [P, P, P, P, U32, U32, U32, C.c_float, P, P, P, P, P, P,
+                               C.c_size_t]),
     "akh_model_new": (ST, [P, C.POINTER(ModelConfigC), C.POINTER(P)]),
     "akh_model_free": (None, [P]),
     "akh_model_num_params": (U32, [P]),
@@ -338,6 +364,42 @@ def _p(x):
     if isinstance(x, DeviceTensor):
         return x.ptr
     return x
+
+
+def q8_cache_bytes(slots: int, max_rows: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of an 8-bit cache's buffer."""
+    lib, n = load(), C.c_size_t()
+    c = Q8CacheC(None, slots, max_rows, kv_heads, head_dim)
+    _check(lib.akh_q8_cache_bytes(C.byref(c), C.byref(n)), "q8_cache_bytes")
+    return n.value
+
+
+def attn_q8_workspace(shape: AttnQ8, cache: "Q8Cache", prefix: "Q8Cache | None" = None) -> int:
+    """Workspace bytes of attn_cached_q8, or of attn_prefix_q8 with `prefix`."""
+    lib, n = load(), C.c_size_t()
+    _check(lib.akh_attn_q8_workspace(C.byref(shape), C.byref(cache.c),
+                                     C.byref(prefix.c) if prefix is not None else None,
+                                     C.byref(n)), "attn_q8_workspace")
+    return n.value
+
+
+def verify_drafts_workspace(batch: int, rows: int, n: int) -> int:
+    """Workspace bytes of verify_drafts."""
+    lib, out = load(), C.c_size_t()
+    _check(lib.akh_verify_drafts_workspace(batch, rows, n, C.byref(out)),
+           "verify_drafts_workspace")
+    return out.value
+
+
+class Q8Cache:
+    """An 8-bit cache: a buffer of its own (zeroed), or the given one
+    (`data`: a DeviceTensor, or a device pointer the caller keeps alive)."""
+
+    def __init__(self, backend: "Backend", slots: int, max_rows: int, kv_heads: int,
+                 head_dim: int, data=None):
+        self.data = data if data is not None else DeviceTensor(
+            backend, q8_cache_bytes(slots, max_rows, kv_heads, head_dim))
+        self.c = Q8CacheC(_p(self.data), slots, max_rows, kv_heads, head_dim)
 
 
 # Backends still open when the interpreter exits are closed (children
@@ -525,6 +587,42 @@ class Backend:
                                             _p(uniforms) if uniforms is not None else None,
                                             _p(out)),
                "sample_rows_noalloc")
+
+
+    # 8-bit caches, attention over them, drafted tokens (device buffers throughout)
+    def cache_write_q8(self, k, v, cache: Q8Cache, batch, rows, src_stride, pos, counts=None):
+        """Quantise the step's K and V rows into the cache."""
+        _check(_lib.akh_cache_write_q8(self.handle, _p(k), _p(v), cache.c, batch, rows, src_stride,
+                                       _p(pos), _p(counts)), "cache_write_q8")
+
+    def cache_read_q8(self, cache: Q8Cache, k, v, batch, rows, dst_stride, pos, counts=None):
+        """The values the cache holds at the step's places (k or v may be None)."""
+        _check(_lib.akh_cache_read_q8(self.handle, cache.c, _p(k), _p(v), batch, rows, dst_stride,
+                                      _p(pos), _p(counts)), "cache_read_q8")
+
+    def attn_cached_q8(self, q, cache: Q8Cache, out, lse, shape: AttnQ8, pos, counts=None,
+                       workspace=None, workspace_bytes=0):
+        """Attention of each sequence's newest rows over its slot of the cache."""
+        _check(_lib.akh_attn_cached_q8(self.handle, _p(q), cache.c, _p(out), _p(lse), shape,
+                                       _p(pos), _p(counts), _p(workspace), workspace_bytes),
+               "attn_cached_q8")
+
+    def attn_prefix_q8(self, q, prefix: Q8Cache, prefix_len, cache: Q8Cache, out, lse,
+                       shape: AttnQ8, pos, counts=None, workspace=None, workspace_bytes=0):
+        """attn_cached_q8 with prefix_len[0] shared rows before every
+        sequence's own."""
+        _check(_lib.akh_attn_prefix_q8(self.handle, _p(q), prefix.c, _p(prefix_len), cache.c,
+                                       _p(out), _p(lse), shape, _p(pos), _p(counts),
+                                       _p(workspace), workspace_bytes), "attn_prefix_q8")
+
+    def verify_drafts(self, target, draft, tokens, batch, rows, n, out_tokens, out_counts,
+                      chance=None, temperature=0.0, counts=None, uniforms=None, workspace=None,
+                      workspace_bytes=0):
+        """Speculative sampling's acceptance of drafted tokens."""
+        _check(_lib.akh_verify_drafts(self.handle, _p(target), _p(draft), _p(tokens), batch, rows,
+                                      n, temperature, _p(counts), _p(uniforms), _p(out_tokens),
+                                      _p(out_counts), _p(chance), _p(workspace),
+                                      workspace_bytes), "verify_drafts")
 
 
 class Graph:

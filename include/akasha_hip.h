@@ -257,6 +257,122 @@ akh_status akh_sample_rows_noalloc(akh_backend* be, const float* logits, uint32_
                                    uint32_t seen_stride, const uint32_t* seen_len,
                                    const double* uniforms, uint32_t* out);
 
+/* ---- 2b. 8-bit caches, attention over them, drafted tokens ---------------
+ *
+ * A batch decodes several drafted tokens a step from a KV cache of 8-bit
+ * codes: akh_cache_write_q8 stores the step's K and V rows, one of the
+ * akh_attn_*_q8 attends from them, akh_verify_drafts keeps the drafts that the
+ * target's distribution allows.  No counterparts in the reference, whose cache
+ * is f32 and per sequence (inference_graphs.rs:511-538; the launchers above).
+ *
+ * What the calls share: sequence b of a batch is slot b of its cache; row t
+ * of sequence b is row b * rows + t of the caller's [batch * rows, stride]
+ * buffers; the sequence's rows of this step are t < min(counts[b], rows)
+ * (counts NULL: all of them), and row t's place in the cache is pos[b] + t.
+ * pos, counts and prefix_len are device arrays read when the kernels run, so
+ * a captured graph follows them as it follows metas.  Every call is queued on
+ * the backend's stream and allocates nothing.  Work for zero sequences or
+ * rows is AKH_OK and does nothing.
+ *
+ * A workspace is device memory of the size its *_workspace function tells,
+ * aligned to 16 bytes, that a call uses until its kernels have run: calls on
+ * one backend (replays of its graphs among them) may share one, calls that
+ * can overlap (other backends) may not.  Its contents need no preparation.
+ */
+
+/* An 8-bit cache: one device buffer of akh_q8_cache_bytes(), aligned to 16
+ * bytes, K codes, then V codes ([slots][kv_heads][cap][row] int8), K exponents, then V
+ * exponents ([slots][kv_heads][cap] int8), where cap is max_rows rounded up
+ * to a multiple of 32 and row is 64 bytes up to head_dim 64, 128 beyond
+ * (codes past head_dim are 0).  A head's row holds code * 2^exponent: the
+ * exponent is the least whole number e >= -126 with max|x| <= 127 * 2^e, the
+ * codes x * 2^-e rounded to nearest, ties to even, so a value is off by at
+ * most 2^(e-1) <= max(max|x| / 127, 2^-127) (what would round to 2^128 takes
+ * the code below, 63 * 2^122).  A head's row with a NaN or an infinity has
+ * exponent -128 and reads back as NaN throughout.  head_dim 1..128,
+ * max_rows <= 2^30. */
+typedef struct {
+  void* data;
+  uint32_t slots, max_rows, kv_heads, head_dim;
+} akh_q8_cache;
+/* Bytes of the buffer (data is not looked at). */
+akh_status akh_q8_cache_bytes(const akh_q8_cache* cache, size_t* bytes);
+/* Quantises the step's K and V rows (f32, head h of a row at h * head_dim;
+ * src_stride >= kv_heads * head_dim floats, so a fused QKV output's columns
+ * will do) and stores them.  Rows whose place is max_rows or more are
+ * dropped; cache rows outside the step are left as they are. */
+akh_status akh_cache_write_q8(akh_backend* be, const float* k, const float* v,
+                              akh_q8_cache cache, uint32_t batch, uint32_t rows,
+                              uint32_t src_stride, const uint32_t* pos, const uint32_t* counts);
+/* The values the cache holds at the step's places, f32, laid out as
+ * akh_cache_write_q8 takes them.  Rows of the buffers that are not the
+ * step's, or whose place is max_rows or more, become zero; columns past
+ * kv_heads * head_dim are left alone.  k or v may be NULL. */
+akh_status akh_cache_read_q8(akh_backend* be, akh_q8_cache cache, float* k, float* v,
+                             uint32_t batch, uint32_t rows, uint32_t dst_stride,
+                             const uint32_t* pos, const uint32_t* counts);
+
+/* Sizes of an attention call.  heads is a multiple of the cache's kv_heads:
+ * query head h reads kv head h / (heads / kv_heads).  Row strides in floats,
+ * at least heads * head_dim.  max_len: the longest pos[b] + rows expected; it
+ * only shapes the launch and its workspace (0: the cache's max_rows), longer
+ * sequences are attended to in full all the same. */
+typedef struct {
+  uint32_t batch, rows, heads, q_stride, out_stride;
+  float scale;
+  uint32_t max_len;
+} akh_attn_q8;
+/* Workspace of akh_attn_cached_q8 (prefix NULL) or akh_attn_prefix_q8; may
+ * be 0. */
+akh_status akh_attn_q8_workspace(const akh_attn_q8* shape, const akh_q8_cache* cache,
+                                 const akh_q8_cache* prefix, size_t* bytes);
+/* out[b, t, h] = sum_j softmax_j(scale q[b, t, h] . k_j) v_j over the cache
+ * rows j <= pos[b] + t, j < max_rows of slot b, and lse[b, t, h] ([batch,
+ * rows, heads], may be NULL) = ln sum_j exp(scale q . k_j).  Rows t >=
+ * counts[b] get zeros and -infinity.  Products in two fp16 terms of q and of
+ * the softmax weights with the exact codes, sums in f32: the accuracy of f32
+ * arithmetic on the cache's values.  NaN and infinities in q and NaN rows of
+ * the cache make the heads that use them NaN.  out may not overlap q. */
+akh_status akh_attn_cached_q8(akh_backend* be, const float* q, akh_q8_cache cache, float* out,
+                              float* lse, akh_attn_q8 shape, const uint32_t* pos,
+                              const uint32_t* counts, void* workspace, size_t workspace_bytes);
+/* akh_attn_cached_q8 where every sequence has the rows j < prefix_len[0] (at
+ * most max_rows) of slot 0 of `prefix` before its own: a prompt that the
+ * batch shares is stored once, and read once for all of a kv head's query rows
+ * (32 at a time).  prefix has the cache's kv_heads and head_dim. */
+akh_status akh_attn_prefix_q8(akh_backend* be, const float* q, akh_q8_cache prefix,
+                              const uint32_t* prefix_len, akh_q8_cache cache, float* out,
+                              float* lse, akh_attn_q8 shape, const uint32_t* pos,
+                              const uint32_t* counts, void* workspace, size_t workspace_bytes);
+
+/* Workspace of akh_verify_drafts. */
+akh_status akh_verify_drafts_workspace(uint32_t batch, uint32_t rows, uint32_t n, size_t* bytes);
+/* Speculative sampling's acceptance rule (Leviathan et al., 2023; Chen et
+ * al., 2023) on device logits.  Sequence b has drafts x_t = tokens[b, t], t < c = min(counts[b],
+ * rows); target is [batch, rows + 1, n] (row t: the logits that choose the
+ * token in x_t's place, row c: the one after the last draft), draft is
+ * [batch, rows, n], the logits x_t was drawn from, or NULL for drafts that
+ * were not drawn (all of their distribution on x_t).  With p_t and q_t
+ * the softmaxes of both at `temperature`, x_t is accepted when
+ * uniforms[b, t] * q_t(x_t) < p_t(x_t) (uniforms: [batch, rows + 1] in
+ * [0, 1)).  out_tokens[b] ([rows + 1]) receives the drafts before the first
+ * one refused, r, and one more token: drawn from max(0, p_r - q_r), or from
+ * p_c if none was refused, as the lowest id whose cumulative weight exceeds
+ * uniforms[b, rows] times the total; entries behind it become UINT32_MAX.
+ * out_counts[b] counts the tokens (r + 1).  chance ([batch, rows], may be
+ * NULL) receives min(1, p_t(x_t) / q_t(x_t)) for t < c and 0 behind.
+ * temperature <= 0: x_t is accepted when it is row t's first maximum, the
+ * last token is its row's first maximum, draft and uniforms are not read.
+ * Probabilities are computed in f64.  A logit that is NaN has weight zero,
+ * a row without weight left (NaN, infinite or -infinite logits only) gives the
+ * first maximum of its numbers (0 if it has none), an id >= n is never
+ * accepted.  A p_r - q_r without weight falls back to p_r. */
+akh_status akh_verify_drafts(akh_backend* be, const float* target, const float* draft,
+                             const uint32_t* tokens, uint32_t batch, uint32_t rows, uint32_t n,
+                             float temperature, const uint32_t* counts, const double* uniforms,
+                             uint32_t* out_tokens, uint32_t* out_counts, float* chance,
+                             void* workspace, size_t workspace_bytes);
+
 /* ---- 3. model weights and the batched session ---------------------------- */
 
 /* ModelConfig (src/config.rs:1-30). */
