@@ -573,10 +573,17 @@ struct AttnQ8Args {
   uint32_t batch, rows, heads, q_stride, out_stride, max_len;
   float scale;
   void* ws;
-  int num_cus;
+  bool q_vec;  // q's rows can be read as float4 (set by the launch)
 };
-size_t attn_q8_workspace_bytes(const AttnQ8Args& a);
-hipError_t launch_attn_q8(const AttnQ8Args& a, hipStream_t s);
+// How an attention call is dealt to blocks, from its sizes alone.
+constexpr uint32_t kAttnMaxSplits = 64;
+struct AttnQ8Plan {
+  uint32_t own_rt, own_groups, own_splits;           // rows a job, jobs, splits of the keys
+  uint32_t prefix_rt, prefix_groups, prefix_splits;  // splits 0: no prefix
+  size_t rows_offset, bytes;  // the workspace: maxima and sums, then rows
+};
+size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix);
+hipError_t launch_attn_q8(AttnQ8Args a, hipStream_t s);
 
 struct VerifyArgs {
   const float* target;     // [batch, rows + 1, n]

@@ -6,6 +6,8 @@
 // the same values whatever order it reads them in.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "common.h"
 #include "kernels.h"
 
@@ -137,72 +139,564 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
   }
 }
 
-// One block per (sequence, row, head): four waves deal the keys of the
-// prefix and of the sequence's own rows among them, a lane holds ROW / 64
-// columns, and the waves' running maxima, sums and weighted rows are joined
-// at the end.
+// ---- attention ---------------------------------------------------------------
+//
+// A job is one kv head's keys of one source (a sequence's slot, or the
+// prefix), a group of the query rows that read them, and one of the splits of
+// those keys.  Its block's waves deal the split's 32-key tiles among them and
+// go through each tile once, with the softmax's running maximum and sum:
+//
+//   S^T = K Q^T      16x16x32 fp16 MFMAs, A = K's codes, B = the rows' q
+//   P^T = 2^(S - m)  in the accumulators' layout, which is already B's
+//   O^T += V^T P^T   A = V's codes by dimension
+//
+// int8 codes are exact in fp16, q and P go in as two fp16 terms each, hi + lo
+// (22 bits).  With at most 8 rows the terms are two columns of one MFMA (PACK:
+// column c is row c's hi, c + 8 its lo); otherwise two MFMAs into one
+// accumulator, 16 rows a tile, NT tiles.
+//
+// Lane l = 16 g + c.  K: the lane holds 16 columns of key c (16 g + 64 u
+// ..), which two MFMA steps contract in that order, q's alike.  S^T: rows
+// (keys) 4 g + r of both 16-key halves, column c.  P^T as B wants keys 8 g
+// + i of a 32-key contraction: keys are taken in the order 4 g + r, 16 + 4 g + r,
+// so P never leaves its lane; V's codes come in the same order, the lane's
+// ROW / 16 consecutive columns of eight keys: column (ROW / 16) c + j is A's
+// row c of MFMA j.
+//
+// The exponents: a key's K scale multiplies its scores, its V scale its
+// weights.  Weights are kept at 2^(x - mt) 2^(ve - eb) with mt (per row) and
+// eb (per wave) such that the largest lies at 2^8, whole powers of two; they
+// may grow to 2^15 before mt and eb move and the accumulators are rescaled
+// (exactly), so most tiles neither join maxima across lanes nor rescale.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Bytes 0, 1 and 2, 3 of four offset codes (code + 128) as fp16 codes: under
+// the exponent byte 0x64 a byte reads 1024 + it.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const h2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+  w ^= 0x80808080u;
+  lo = __builtin_bit_cast(
+      uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + off);
+  hi = __builtin_bit_cast(
+      uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + off);
+}
+__device__ __forceinline__ f16x8 codes8_f16(uint32_t a, uint32_t b) {
+  uint4 r;
+  codes_f16(a, r.x, r.y);
+  codes_f16(b, r.z, r.w);
+  return f16x8_of(r);
+}
+// Byte J of two dwords as a pair of fp16 codes.
+template <int J>
+__device__ __forceinline__ uint32_t pair_f16(uint32_t a, uint32_t b) {
+  const h2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+  const uint32_t w = __builtin_amdgcn_perm(b, a, 0x0C040C00u + J * 0x00010001u) ^ 0x64806480u;
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, w) + off);
+}
+
+// Two floats of at most 2^15 as hi + lo fp16 pairs: hi truncated to 11
+// bits, lo the next 11 (their sum within 2^-21, or 2^-24 below fp16's normal
+// range).
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
+  const float hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ha, hb));
+  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - ha, b - hb));
+}
+
+__device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+
+// What one 32-key tile's lane loads.
 template <int ROW>
-__global__ __launch_bounds__(256) void k_attn_q8(AttnQ8Args a) {
-  constexpr int D = ROW / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t h = blockIdx.x % a.heads;
-  const uint64_t bt = blockIdx.x / a.heads;
-  const uint32_t b = (uint32_t)(bt / a.rows), t = (uint32_t)(bt % a.rows);
-  const uint32_t kvh = h / (a.heads / a.c.kv_heads);
-  float* out = a.out + bt * a.out_stride + (size_t)h * a.c.head_dim;
-  const bool live = t < step_rows(a.counts, b, a.rows);
-  const uint32_t own =
-      live ? (uint32_t)min<uint64_t>((uint64_t)a.pos[b] + t + 1, a.c.max_rows) : 0;
-  const uint32_t ahead = live && a.prefix_len ? min(*a.prefix_len, a.pre.max_rows) : 0;
-  float q[D], acc[D];
+struct Tile {
+  uint4 k[2][ROW / 64];
+  uint32_t v[8][ROW / 64];
+  uint32_t ke[2], ve[2];
+};
+
+template <int ROW>
+__device__ __forceinline__ void load_tile(Tile<ROW>& t, const int8_t* k, const int8_t* v,
+                                          const int8_t* ke, const int8_t* ve, uint32_t key0,
+                                          int g, int c) {
+  const int8_t* kp = k + (size_t)(key0 + c) * ROW + 16 * g;
 #pragma unroll
-  for (int i = 0; i < D; ++i) {
-    const int col = lane * D + i;
-    q[i] = col < (int)a.c.head_dim ? a.q[bt * a.q_stride + (size_t)h * a.c.head_dim + col] : 0.f;
-    acc[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (uint64_t j = wave; j < (uint64_t)ahead + own; j += 4) {
-    const bool first = j < ahead;
-    const Q8Cache& c = first ? a.pre : a.c;
-    const size_t row = ((size_t)(first ? 0 : b) * c.kv_heads + kvh) * c.cap + (first ? j : j - ahead);
-    float s = 0.f, vv[D];
+  for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-    for (int i = 0; i < D; ++i) {
-      s = fmaf(q[i], (float)c.k[row * ROW + lane * D + i], s);
-      vv[i] = (float)c.v[row * ROW + lane * D + i];
+    for (int u = 0; u < ROW / 64; ++u)
+      t.k[hh][u] = *reinterpret_cast<const uint4*>(kp + hh * 16 * ROW + u * 64);
+  const int8_t* vp = v + (size_t)(key0 + 4 * g) * ROW + c * (ROW / 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int8_t* p = vp + ((i & 3) + (i >> 2) * 16) * ROW;
+    if constexpr (ROW == 64) {
+      t.v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      t.v[i][0] = w.x;
+      t.v[i][1] = w.y;
     }
-    s = wave_sum(s) * exp_value(c.ke[row]) * a.scale;
-    const float mn = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - mn);
-    const float p = mn == -INFINITY && s == -INFINITY ? 0.f : expf(s - mn);
-    const float w = p * exp_value(c.ve[row]);
-    l = l * keep + p;
-#pragma unroll
-    for (int i = 0; i < D; ++i) acc[i] = acc[i] * keep + w * vv[i];
-    m = mn;
-  }
-  __shared__ float sm[4], sl[4], sa[4][ROW];
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
   }
 #pragma unroll
-  for (int i = 0; i < D; ++i) sa[wave][lane * D + i] = acc[i];
+  for (int hh = 0; hh < 2; ++hh) {
+    t.ke[hh] = *reinterpret_cast<const uint32_t*>(ke + key0 + 16 * hh + 4 * g);
+    t.ve[hh] = *reinterpret_cast<const uint32_t*>(ve + key0 + 16 * hh + 4 * g);
+  }
+}
+
+// One query row of a job.
+struct RowRef {
+  uint64_t bt;     // row of q and out
+  uint32_t head;
+  uint32_t limit;  // keys it sees
+  bool live;       // it is the step's (otherwise it sees no key)
+};
+
+// Row r of a job's rows (SHARED: of every sequence), G query heads each.
+template <bool SHARED>
+__device__ __forceinline__ RowRef row_ref(const AttnQ8Args& a, uint32_t b, uint32_t kvh,
+                                          uint32_t r, uint32_t prefix_keys) {
+  const uint32_t G = a.heads / a.c.kv_heads;
+  RowRef x;
+  uint32_t t = r / G;
+  x.head = kvh * G + r % G;
+  if constexpr (SHARED) {
+    b = t / a.rows;
+    t -= b * a.rows;
+  }
+  x.live = b < a.batch && t < step_rows(a.counts, b, a.rows);
+  x.limit = 0;
+  if (x.live)
+    x.limit = SHARED ? prefix_keys
+                     : (uint32_t)min<uint64_t>((uint64_t)a.pos[b] + t + 1, a.c.max_rows);
+  x.bt = (uint64_t)b * a.rows + t;
+  return x;
+}
+
+// q of one row as MFMA B operands, hi and lo, scaled by scale log2(e) and by
+// 2^-e to a largest magnitude in [2^13, 2^14); returns 2^e, NaN for a row
+// with a NaN or an infinity.
+template <int ROW>
+__device__ __forceinline__ float load_q(const AttnQ8Args& a, const RowRef& r, int g, f16x8* hi,
+                                        f16x8* lo) {
+  constexpr int KS = ROW / 32;
+  const float* q = a.q + r.bt * a.q_stride + (size_t)r.head * a.c.head_dim;
+  const float cs = (float)((double)a.scale * 1.4426950408889634);
+  const int hd = (int)a.c.head_dim;
+  float x[KS][8];
+  float top = 0.f, sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int d0 = (s >> 1) * 64 + 16 * g + 8 * (s & 1);
+    if (a.q_vec && d0 + 8 <= hd && r.limit) {
+      const float4 u = *reinterpret_cast<const float4*>(q + d0);
+      const float4 w = *reinterpret_cast<const float4*>(q + d0 + 4);
+      x[s][0] = u.x, x[s][1] = u.y, x[s][2] = u.z, x[s][3] = u.w;
+      x[s][4] = w.x, x[s][5] = w.y, x[s][6] = w.z, x[s][7] = w.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] = r.limit && d0 + i < hd ? q[d0 + i] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[s][i] *= cs;
+      top = fmaxf(top, fabsf(x[s][i]));
+      sum += x[s][i] * 0.f;  // NaN where anything is not finite
+    }
+  }
+  top = xor_max<32>(xor_max<16>(top));
+  sum = xor_sum<32>(xor_sum<16>(sum));
+  // top = 1.m 2^(E - 127); times 2^(140 - E) it is 1.m 2^13 (E at least 15, so
+  // that 2^e stays a normal number's inverse; smaller rows keep small terms).
+  const int E = max(15, (int)(__float_as_uint(top) >> 23));
+  const float s1 = ldexpf(1.f, 140 - E), back = ldexpf(1.f, E - 140);
+  const bool ok = sum == 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      split2(ok ? x[s][2 * i] * s1 : 0.f, ok ? x[s][2 * i + 1] * s1 : 0.f, h[i], l[i]);
+    hi[s] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
+    lo[s] = f16x8_of(make_uint4(l[0], l[1], l[2], l[3]));
+  }
+  return ok ? back : __int_as_float(0x7FC00000);
+}
+
+// Partial results of a row: maximum (log2), sum and normalised weighted row
+// of each part; the prefix's splits first, then the own rows'.
+struct PartMl {
+  float m, l;
+};
+__device__ __forceinline__ size_t row_id(const AttnQ8Args& a, const RowRef& r) {
+  return r.bt * a.heads + r.head;
+}
+
+// SHARED: the prefix's keys for the rows of all sequences, as partial results.
+// Otherwise a sequence's own keys; with one split (and the prefix's partial
+// results, where there are) the block writes the output itself.
+template <int ROW, int NT, bool PACK, int WAVES, bool SHARED>
+__global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan pl) {
+  constexpr int KS = ROW / 32;           // MFMA steps of a score
+  constexpr int DT = ROW / 16;           // MFMAs of 16 output columns
+  constexpr int RT = PACK ? 8 : 16 * NT; // rows of a job
+  static_assert(!PACK || NT == 1, "one packed tile");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, c = lane & 15;
+  uint32_t id = blockIdx.x;
+  const uint32_t splits = SHARED ? pl.prefix_splits : pl.own_splits;
+  const uint32_t groups = SHARED ? pl.prefix_groups : pl.own_groups;
+  const uint32_t group = id % groups;
+  id /= groups;
+  const uint32_t kvh = id % a.c.kv_heads;
+  id /= a.c.kv_heads;
+  const uint32_t split = id % splits;
+  const uint32_t b = id / splits;  // 0 when SHARED
+  const uint32_t G = a.heads / a.c.kv_heads;
+  const uint32_t nrows = SHARED ? a.batch * a.rows * G : a.rows * G;
+  const uint32_t row0 = group * RT;
+  const Q8Cache& src = SHARED ? a.pre : a.c;
+  const uint32_t pkeys = a.prefix_len ? min(*a.prefix_len, a.pre.max_rows) : 0;
+
+  RowRef ref[NT];
+  uint32_t most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const uint32_t r = row0 + n * 16 + (PACK ? c & 7 : c);
+    ref[n] = row_ref<SHARED>(a, b, kvh, min(r, nrows - 1), pkeys);
+    if (r >= nrows) ref[n].limit = 0;
+    most = max(most, ref[n].limit);
+    if (ref[n].limit) least = min(least, ref[n].limit);
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+    least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+  }
+  most = __builtin_amdgcn_readfirstlane(most);
+  least = __builtin_amdgcn_readfirstlane(least);
+
+  f16x8 qh[NT][KS], ql[PACK ? 1 : NT][KS];
+  float qf[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if constexpr (PACK) {
+      f16x8 lo[KS];
+      qf[n] = load_q<ROW>(a, ref[n], g, qh[n], lo);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qh[n][s] = c < 8 ? qh[n][s] : lo[s];
+    } else {
+      qf[n] = load_q<ROW>(a, ref[n], g, qh[n], ql[n]);
+    }
+  }
+
+  f32x4 acc[NT][DT];
+  float mt[NT], top_x[NT], top_w[NT], l[NT];
+  int eb = -126;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    mt[n] = 0.f;
+    top_x[n] = top_w[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int j = 0; j < DT; ++j) acc[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // The split's tiles [t0, t1), the waves' in turn.
+  const uint32_t tiles = (most + 31) / 32;
+  const uint32_t per = (tiles + splits - 1) / splits;
+  const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
+  const size_t base = ((size_t)(SHARED ? 0 : b) * src.kv_heads + kvh) * src.cap;
+  const int8_t* kp = src.k + base * ROW;
+  const int8_t* vp = src.v + base * ROW;
+  const int8_t* kep = src.ke + base;
+  const int8_t* vep = src.ve + base;
+  Tile<ROW> cur;
+  uint32_t t = t0 + wave;
+  if (t < t1) load_tile<ROW>(cur, kp, vp, kep, vep, t * 32, g, c);
+  bool fresh = true;
+  for (; t < t1; t += WAVES) {
+    Tile<ROW> next;
+    load_tile<ROW>(next, kp, vp, kep, vep, min(t + WAVES, t1 - 1) * 32, g, c);
+
+    f32x4 d[NT][2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[n][hh] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint4 w = cur.k[hh][s >> 1];
+        const f16x8 ka = (s & 1) ? codes8_f16(w.z, w.w) : codes8_f16(w.x, w.y);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          d[n][hh] = mfma16(ka, qh[n][s], d[n][hh]);
+          if constexpr (!PACK) d[n][hh] = mfma16(ka, ql[n][s], d[n][hh]);
+        }
+      }
+    }
+    // Exponents of the lane's eight keys.
+    const bool tail = t * 32 + 32 > least;
+    const uint32_t key0 = t * 32 + 4 * g;  // + i, and + 12 + i from the fifth on
+    int ek[8], ev[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ek[i] = byte_s(cur.ke[i >> 2], i & 3);
+      ev[i] = byte_s(cur.ve[i >> 2], i & 3);
+    }
+    if (tail) {  // behind the rows' last key there may be anything
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (key0 + i + (i >> 2) * 12 >= most) ek[i] = ev[i] = -126;
+    }
+    int low = 0, high = -126;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      low = min(low, min(ek[i], ev[i]));
+      high = max(high, ev[i]);
+    }
+    const bool nans = __any(low == kNanExp);
+    // Scores, in units of ln 2.
+    float x[NT][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float kf = __int_as_float((ek[i] + 127) << 23);
+      if (nans) kf = ek[i] == kNanExp ? __int_as_float(0x7FC00000) : kf;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float s = d[n][i >> 2][i & 3];
+        if constexpr (PACK) s += dpp_f32<0x128>(s);  // row_ror:8, the other term's column
+        x[n][i] = s * (kf * qf[n]);
+        if (tail) x[n][i] = key0 + i + (i >> 2) * 12 >= ref[n].limit ? -INFINITY : x[n][i];
+      }
+    }
+    uint32_t ph[NT][4], plo[NT][4];
+    float add[NT];
+    bool redo = fresh;
+#pragma unroll 1
+    for (int round = 0; round < 2; ++round) {  // the second one's levels fit
+      if (redo) {
+        // New levels: the largest x + ve of a row at 2^8.
+        int e1 = high;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) e1 = max(e1, __shfl_xor(e1, o, 64));
+        const int eb1 = max(eb, __builtin_amdgcn_readfirstlane(e1));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float mx = -INFINITY, mw = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            mx = fmaxf(mx, x[n][i]);
+            mw = fmaxf(mw, x[n][i] + (float)ev[i]);
+          }
+          mx = xor_max<32>(xor_max<16>(mx));
+          mw = xor_max<32>(xor_max<16>(mw));
+          top_x[n] = fmaxf(top_x[n], ceilf(mx));
+          top_w[n] = fmaxf(top_w[n], ceilf(mw));
+          float m1 = fmaxf(top_w[n] - (float)eb1 - 8.f, top_x[n] - 100.f);
+          if (m1 == -INFINITY) m1 = 0.f;  // no key yet
+          const float keep = fresh ? 0.f : __builtin_amdgcn_exp2f(mt[n] - m1);
+          const float keep_o =
+              fresh ? 0.f : __builtin_amdgcn_exp2f(mt[n] - m1 + (float)(eb - eb1));
+          l[n] *= keep;
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[n][j][r] *= keep_o;
+          mt[n] = m1;
+        }
+        eb = eb1;
+        fresh = false;
+      }
+      bool over = high - eb > 100;
+      float vf[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        vf[i] = ldexpf(1.f, ev[i] - eb);
+        if (nans) vf[i] = ev[i] == kNanExp ? __int_as_float(0x7FC00000) : vf[i];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[8], big = 0.f;
+        add[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = __builtin_amdgcn_exp2f(x[n][i] - mt[n]);
+          add[n] += p;
+          w[i] = p * vf[i];
+          if (tail) w[i] = key0 + i + (i >> 2) * 12 >= ref[n].limit ? 0.f : w[i];
+          big = fmaxf(big, w[i]);
+        }
+        over |= big > 32768.f || add[n] > 0x1p110f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split2(w[2 * i], w[2 * i + 1], ph[n][i], plo[n][i]);
+      }
+      redo = __any(over);
+      if (!redo) break;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) l[n] += add[n];
+    // O^T += V^T P^T.
+#pragma unroll
+    for (int j = 0; j < DT; ++j) {
+      constexpr int W = ROW / 64;
+      const int wd = j / 4;
+      uint32_t p4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v0 = cur.v[2 * i][W == 1 ? 0 : wd], v1 = cur.v[2 * i + 1][W == 1 ? 0 : wd];
+        switch (j & 3) {
+          case 0: p4[i] = pair_f16<0>(v0, v1); break;
+          case 1: p4[i] = pair_f16<1>(v0, v1); break;
+          case 2: p4[i] = pair_f16<2>(v0, v1); break;
+          default: p4[i] = pair_f16<3>(v0, v1); break;
+        }
+      }
+      const f16x8 va = f16x8_of(make_uint4(p4[0], p4[1], p4[2], p4[3]));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (PACK) {
+          const bool hi = c < 8;
+          acc[n][j] = mfma16(va, f16x8_of(make_uint4(hi ? ph[n][0] : plo[n][0], hi ? ph[n][1] : plo[n][1],
+                                                     hi ? ph[n][2] : plo[n][2], hi ? ph[n][3] : plo[n][3])),
+                             acc[n][j]);
+        } else {
+          acc[n][j] = mfma16(va, f16x8_of(make_uint4(ph[n][0], ph[n][1], ph[n][2], ph[n][3])), acc[n][j]);
+          acc[n][j] = mfma16(va, f16x8_of(make_uint4(plo[n][0], plo[n][1], plo[n][2], plo[n][3])),
+                             acc[n][j]);
+        }
+      }
+    }
+    cur = next;
+  }
+
+  // Join the waves: each one's row normalised, weighted by its sum.
+  constexpr int RS = ROW + 4;
+  constexpr int MAXP = kAttnMaxSplits;
+  __shared__ float so[WAVES][RT][RS];
+  __shared__ PartMl sml[WAVES][RT];
+  __shared__ float sw[RT][WAVES + (SHARED ? 0 : MAXP)];
+  __shared__ float2 sfin[RT];  // maximum and sum of a row over all its parts
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float total = xor_sum<32>(xor_sum<16>(l[n]));
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const int row = n * 16 + c;
+    const bool mine = !PACK || c < 8;
+    if (g == 0 && mine) sml[wave][row] = {total == 0.f ? -INFINITY : mt[n], total};
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float o = acc[n][j][r];
+        if constexpr (PACK) o += dpp_f32<0x128>(o);
+        if (mine && ref[n].limit) so[wave][row][(4 * g + r) * DT + j] = ldexpf(o * inv, eb);
+      }
+  }
   __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  float f[4], total = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    f[w] = sm[w] == -INFINITY ? (sl[w] == sl[w] ? 0.f : 1.f) : expf(sm[w] - top);
-    total += sl[w] * f[w];
+  const bool final = !SHARED && pl.own_splits == 1;
+  const uint32_t extra = final ? pl.prefix_splits : 0;
+  const PartMl* ml = reinterpret_cast<const PartMl*>(a.ws);
+  float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
+  const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
+  if (threadIdx.x < RT) {
+    const int row = threadIdx.x;
+    const RowRef x = row_ref<SHARED>(a, b, kvh, min(row0 + row, nrows - 1), pkeys);
+    float m = -INFINITY;
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, sml[w][row].m);
+    const bool live = row0 + row < nrows && x.live;
+    if (live)
+      for (uint32_t e = 0; e < extra; ++e) m = fmaxf(m, ml[row_id(a, x) * nparts + e].m);
+    float total = 0.f;
+    for (int w = 0; w < WAVES; ++w) {
+      const PartMl y = sml[w][row];
+      const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
+      sw[row][w] = f;
+      total += f;
+    }
+    if constexpr (!SHARED)
+      for (uint32_t e = 0; live && e < extra; ++e) {
+        const PartMl y = ml[row_id(a, x) * nparts + e];
+        const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
+        sw[row][WAVES + e] = f;
+        total += f;
+      }
+    sfin[row] = make_float2(m, total);
   }
-  if (threadIdx.x < a.c.head_dim) {
-    float x = 0.f;
-    for (int w = 0; w < 4; ++w) x += sa[w][threadIdx.x] * f[w];
-    out[threadIdx.x] = own || ahead ? x / total : 0.f;
+  __syncthreads();
+  const uint32_t hd = a.c.head_dim;
+  const uint32_t rows_here = min((uint32_t)RT, nrows - row0);
+  const uint32_t at = SHARED ? split : pl.prefix_splits + split;
+  for (uint32_t e = threadIdx.x; e < rows_here * ROW; e += 64 * WAVES) {
+    const uint32_t row = e / ROW, col = e % ROW;
+    if (col >= hd) continue;
+    const RowRef x = row_ref<SHARED>(a, b, kvh, row0 + row, pkeys);
+    const float2 fin = sfin[row];
+    float o = 0.f;
+    if (x.live && fin.y != 0.f) {
+      for (int w = 0; w < WAVES; ++w)
+        if (sw[row][w] != 0.f) o += sw[row][w] * so[w][row][col];
+      if constexpr (!SHARED)
+        for (uint32_t p = 0; p < extra; ++p) {
+          const float f = sw[row][WAVES + p];
+          if (f != 0.f) o += f * po[(row_id(a, x) * nparts + p) * ROW + col];
+        }
+      o /= fin.y;
+    }
+    if (final) {
+      a.out[x.bt * a.out_stride + (size_t)x.head * hd + col] = x.live ? o : 0.f;
+      if (col == 0 && a.lse)
+        a.lse[row_id(a, x)] =
+            x.live && fin.y != 0.f ? (fin.x + log2f(fin.y)) * 0.6931471805599453f : -INFINITY;
+    } else if (x.live) {
+      po[(row_id(a, x) * nparts + at) * ROW + col] = o;
+      if (col == 0)
+        const_cast<PartMl*>(ml)[row_id(a, x) * nparts + at] = {fin.y == 0.f ? -INFINITY : fin.x, fin.y};
+    }
   }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[bt * a.heads + h] = own || ahead ? top + logf(total) : -INFINITY;
+}
+
+// Joins a row's partial results: one wave per row and head.
+template <int ROW>
+__global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan pl) {
+  const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (uint64_t)a.batch * a.rows * a.heads) return;
+  const int lane = threadIdx.x & 63;
+  const uint64_t bt = id / a.heads;
+  const uint32_t b = (uint32_t)(bt / a.rows), t = (uint32_t)(bt % a.rows);
+  float* out = a.out + bt * a.out_stride + (id % a.heads) * a.c.head_dim;
+  const uint32_t n = pl.prefix_splits + pl.own_splits;
+  const PartMl* ml = reinterpret_cast<const PartMl*>(a.ws) + id * n;
+  const float* po = reinterpret_cast<const float*>(static_cast<const char*>(a.ws) + pl.rows_offset) +
+                    id * n * ROW;
+  const bool live = t < step_rows(a.counts, b, a.rows);
+  float m = -INFINITY, total = 0.f, o[ROW / 64] = {};
+  if (live) {
+    for (uint32_t p = 0; p < n; ++p) m = fmaxf(m, ml[p].m);
+    for (uint32_t p = 0; p < n; ++p) {
+      const PartMl y = ml[p];
+      if (y.l == 0.f) continue;
+      const float f = y.l * __builtin_amdgcn_exp2f(y.m - m);
+      total += f;
+#pragma unroll
+      for (int i = 0; i < ROW / 64; ++i) {
+        const uint32_t col = lane + 64 * i;
+        if (col < a.c.head_dim) o[i] += f * po[(size_t)p * ROW + col];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROW / 64; ++i) {
+    const uint32_t col = lane + 64 * i;
+    if (col < a.c.head_dim) out[col] = total == 0.f ? 0.f : o[i] / total;
+  }
+  if (lane == 0 && a.lse)
+    a.lse[id] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.6931471805599453f;
 }
 
 uint64_t div_up(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
@@ -239,12 +733,71 @@ hipError_t launch_cache_read_q8(const Q8Cache& c, float* k, float* v, uint32_t b
   return hipGetLastError();
 }
 
-size_t attn_q8_workspace_bytes(const AttnQ8Args&) { return 0; }
+namespace {
 
-hipError_t launch_attn_q8(const AttnQ8Args& a, hipStream_t s) {
-  const dim3 grid((uint32_t)((uint64_t)a.batch * a.rows * a.heads));
-  hipLaunchKernelGGL(a.c.row == 128 ? k_attn_q8<128> : k_attn_q8<64>, grid, dim3(256), 0, s, a);
+// Rows of a job: 8 in packed columns, else 16 or 32.
+uint32_t rows_per_job(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
+AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
+  AttnQ8Plan p{};
+  const uint64_t G = a.heads / a.c.kv_heads;
+  const uint64_t own = a.rows * G, all = own * a.batch;
+  p.own_rt = rows_per_job(own);
+  p.own_groups = (uint32_t)div_up(own, p.own_rt);
+  const uint64_t jobs = (uint64_t)a.batch * a.c.kv_heads * p.own_groups;
+  const uint64_t want = 1024, tiles = div_up(a.max_len, 32);
+  auto splits = [&](uint64_t jobs, uint64_t tiles) {
+    const uint64_t by_work = tiles / 16;  // four tiles a wave at least
+    return (uint32_t)std::max<uint64_t>(
+        1, std::min<uint64_t>({kAttnMaxSplits, by_work, div_up(want, jobs)}));
+  };
+  p.own_splits = splits(jobs, tiles);
+  if (prefix) {
+    p.prefix_rt = rows_per_job(all);
+    p.prefix_groups = (uint32_t)div_up(all, p.prefix_rt);
+    p.prefix_splits = splits((uint64_t)a.c.kv_heads * p.prefix_groups, div_up(a.pre.max_rows, 32));
+  }
+  const uint64_t parts = p.prefix_splits + (p.own_splits > 1 ? p.own_splits : 0);
+  const uint64_t ids = (uint64_t)a.batch * a.rows * a.heads;
+  p.rows_offset = div_up(ids * parts * sizeof(PartMl), 16) * 16;
+  p.bytes = parts ? p.rows_offset + ids * parts * a.c.row * sizeof(float) : 0;
+  return p;
+}
+
+template <int ROW, bool SHARED>
+void launch_parts(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
+  const uint32_t rt = SHARED ? p.prefix_rt : p.own_rt;
+  const dim3 grid(SHARED ? p.prefix_groups * a.c.kv_heads * p.prefix_splits
+                         : a.batch * p.own_splits * a.c.kv_heads * p.own_groups);
+  if (rt == 8)
+    hipLaunchKernelGGL((k_attn_q8<ROW, 1, true, 4, SHARED>), grid, dim3(256), 0, s, a, p);
+  else if (rt == 16)
+    hipLaunchKernelGGL((k_attn_q8<ROW, 1, false, 4, SHARED>), grid, dim3(256), 0, s, a, p);
+  else
+    hipLaunchKernelGGL((k_attn_q8<ROW, 2, false, 4, SHARED>), grid, dim3(256), 0, s, a, p);
+}
+
+template <int ROW>
+hipError_t launch_attn(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
+  if (p.prefix_splits) launch_parts<ROW, true>(a, p, s);
+  launch_parts<ROW, false>(a, p, s);
+  if (p.own_splits > 1)
+    hipLaunchKernelGGL((k_attn_q8_join<ROW>),
+                       dim3((uint32_t)div_up((uint64_t)a.batch * a.rows * a.heads, 4)), dim3(256),
+                       0, s, a, p);
   return hipGetLastError();
+}
+
+}  // namespace
+
+size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix) {
+  return a.batch && a.rows ? attn_q8_plan(a, prefix).bytes : 0;
+}
+
+hipError_t launch_attn_q8(AttnQ8Args a, hipStream_t s) {
+  const AttnQ8Plan p = attn_q8_plan(a, a.prefix_len != nullptr);
+  a.q_vec = vec4(a.q, a.q_stride, a.c.head_dim);
+  return a.c.row == 128 ? launch_attn<128>(a, p, s) : launch_attn<64>(a, p, s);
 }
 
 }  // namespace akh

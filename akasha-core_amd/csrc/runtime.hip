@@ -724,7 +724,7 @@ akh_status q8_rows_args(const akh_q8_cache& cache, uint32_t batch, uint32_t rows
 
 // Checks of an attention call's sizes, as kernel arguments.
 akh_status attn_q8_args(const akh_attn_q8& s, const akh_q8_cache& cache,
-                        const akh_q8_cache* prefix, int num_cus, AttnQ8Args* a) {
+                        const akh_q8_cache* prefix, AttnQ8Args* a) {
   akh_status st = q8_parts(cache, &a->c, nullptr);
   if (st == AKH_OK && prefix) st = q8_parts(*prefix, &a->pre, nullptr);
   if (st != AKH_OK) return st;
@@ -746,7 +746,6 @@ akh_status attn_q8_args(const akh_attn_q8& s, const akh_q8_cache& cache,
   a->out_stride = s.out_stride;
   a->scale = s.scale;
   a->max_len = s.max_len && s.max_len < a->c.max_rows ? s.max_len : a->c.max_rows;
-  a->num_cus = num_cus;
   return AKH_OK;
 }
 
@@ -755,7 +754,7 @@ akh_status attn_q8(akh_backend* be, const float* q, const akh_q8_cache* prefix,
                    const akh_attn_q8& shape, const uint32_t* pos, const uint32_t* counts,
                    void* workspace, size_t workspace_bytes) {
   AttnQ8Args a{};
-  akh_status st = attn_q8_args(shape, cache, prefix, be->num_cus, &a);
+  akh_status st = attn_q8_args(shape, cache, prefix, &a);
   if (st != AKH_OK) return st;
   CHECK_ARG(q && out && pos, "q8 attention: NULL buffer");
   CHECK_ARG(cache.data && aligned16(cache.data) &&
@@ -769,7 +768,7 @@ akh_status attn_q8(akh_backend* be, const float* q, const akh_q8_cache* prefix,
   a.pos = pos;
   a.counts = counts;
   a.ws = workspace;
-  const size_t need = attn_q8_workspace_bytes(a);
+  const size_t need = attn_q8_workspace_bytes(a, prefix != nullptr);
   CHECK_ARG(!need || (workspace && aligned16(workspace) && workspace_bytes >= need),
             "q8 attention: workspace missing, unaligned or smaller than akh_attn_q8_workspace");
   DeviceScope scope(be->device);
@@ -820,9 +819,9 @@ extern "C" akh_status akh_attn_q8_workspace(const akh_attn_q8* shape, const akh_
                                             const akh_q8_cache* prefix, size_t* bytes) {
   CHECK_ARG(shape && cache && bytes, "akh_attn_q8_workspace: NULL argument");
   AttnQ8Args a{};
-  akh_status st = attn_q8_args(*shape, *cache, prefix, 256, &a);
+  akh_status st = attn_q8_args(*shape, *cache, prefix, &a);
   if (st != AKH_OK) return st;
-  *bytes = attn_q8_workspace_bytes(a);
+  *bytes = attn_q8_workspace_bytes(a, prefix != nullptr);
   return AKH_OK;
 }
 

@@ -136,7 +136,7 @@ def _attend(pkg, be, q, cache, pos, counts, scale, prefix=None, prefix_len=0, ma
     lse = be.tensor(np.full(batch * rows * heads, 3.25, np.float32)) if want_lse else None
     shape = h.AttnQ8(batch, rows, heads, stride, stride, scale, max_len)
     size = h.attn_q8_workspace(shape, cache, prefix)
-    ws = be.tensor(np.full(size + 4, 0xA5, np.uint8))  # its contents need no preparation
+    ws = be.tensor(np.full(size + 4, 0xFF, np.uint8))  # NaN: its contents need no preparation
     dp, dc = _u32(be, pos), None if counts is None else _u32(be, counts)
     if prefix is None:
         be.attn_cached_q8(dq, cache, do, lse, shape, dp, dc, ws, size)

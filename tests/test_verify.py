@@ -109,7 +109,7 @@ def run(pkg, be, target, draft, tokens, temperature, uniforms, counts, want_chan
     n = target.shape[-1]
     up = lambda a, t: be.tensor(np.ascontiguousarray(a, t))  # noqa: E731
     size = h.verify_drafts_workspace(batch, rows, n)
-    ws = be.tensor(np.full(size, 0xA5, np.uint8))
+    ws = be.tensor(np.full(size, 0xFF, np.uint8))
     out, kept = be.zeros(batch * (rows + 1), np.uint32), be.zeros(batch, np.uint32)
     chance = be.tensor(np.full(max(1, batch * rows), 9.0, np.float32)) if want_chance else None
     be.verify_drafts(up(target, np.float32), None if draft is None else up(draft, np.float32),
