@@ -573,7 +573,7 @@ struct AttnQ8Args {
   uint32_t batch, rows, heads, q_stride, out_stride, max_len;
   float scale;
   void* ws;
-  bool q_vec;  // q's rows can be read as float4 (set by the launch)
+  bool q_vec, out_vec;  // rows of q and out as float4 (set by the launch)
 };
 // How an attention call is dealt to blocks, from its sizes alone.
 constexpr uint32_t kAttnMaxSplits = 64;

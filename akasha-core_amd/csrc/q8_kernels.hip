@@ -337,6 +337,250 @@ __device__ __forceinline__ size_t row_id(const AttnQ8Args& a, const RowRef& r) {
   return r.bt * a.heads + r.head;
 }
 
+// A wave's rows on their way over the keys.
+template <int ROW, int NT>
+struct RowsState {
+  f32x4 acc[NT][ROW / 16];
+  float mt[NT], top_x[NT], top_w[NT], l[NT];
+  int eb;
+  bool fresh;
+
+  __device__ __forceinline__ void init() {
+    eb = -126;
+    fresh = true;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      mt[n] = 0.f;
+      top_x[n] = top_w[n] = -INFINITY;
+      l[n] = 0.f;
+#pragma unroll
+      for (int j = 0; j < ROW / 16; ++j) acc[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+};
+
+// One tile of 32 keys: kfrag(hh, s) and vfrag(j) give K's and V's A operands,
+// ke / ve the lane's exponents.  limit: keys a row sees; least and most of
+// all rows' (of those that see any) decide whether the tile needs the mask.
+template <int ROW, int NT, bool PACK, class KF, class VF>
+__device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*qh)[ROW / 32],
+                                          const f16x8 (*ql)[ROW / 32], const float* qf,
+                                          const uint32_t* limit, uint32_t least, uint32_t most,
+                                          uint32_t tile, int g, int c, const uint32_t* ke,
+                                          const uint32_t* ve, KF kfrag, VF vfrag) {
+  constexpr int KS = ROW / 32, DT = ROW / 16;
+  f32x4 d[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {  // both halves' products in turn: no MFMA waits for the last one
+    const f16x8 k0 = kfrag(0, s), k1 = kfrag(1, s);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      d[n][0] = mfma16(k0, qh[n][s], d[n][0]);
+      d[n][1] = mfma16(k1, qh[n][s], d[n][1]);
+    }
+    if constexpr (!PACK) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        d[n][0] = mfma16(k0, ql[n][s], d[n][0]);
+        d[n][1] = mfma16(k1, ql[n][s], d[n][1]);
+      }
+    }
+  }
+  // The rare cases are branches of their own that patch what the common path
+  // made (the empty asm keeps them branches).
+  const uint32_t key0 = tile * 32 + 4 * g;  // + i, and + 12 + i from the fifth on
+  uint32_t ek[2] = {ke[0], ke[1]}, ev[2] = {ve[0], ve[1]};
+  const bool tail = tile * 32 + 32 > least;
+  if (tail) {  // behind the rows' last key the exponents may be anything
+    asm volatile("");
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int left = (int)min(most, key0 + 16 * hh + 4) - (int)(key0 + 16 * hh);
+      const uint32_t keep = left <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * left);
+      ek[hh] = (ek[hh] & keep) | (0x82828282u & ~keep);
+      ev[hh] = (ev[hh] & keep) | (0x82828282u & ~keep);
+    }
+  }
+  auto ve_of = [&](int i) { return byte_s(ev[i >> 2], i & 3); };
+  int high = -126;
+  uint32_t bad = 0;  // a byte 0x80 is kNanExp
+#pragma unroll
+  for (int i = 0; i < 8; ++i) high = max(high, ve_of(i));
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh) {
+    const uint32_t x = ek[hh] ^ 0x80808080u, y = ev[hh] ^ 0x80808080u;
+    bad |= (x - 0x01010101u) & ~x;
+    bad |= (y - 0x01010101u) & ~y;
+  }
+  float w[NT][8], add[NT];  // scores (in units of ln 2 once scaled), then weights
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float kf = __int_as_float((byte_s(ek[i >> 2], i & 3) + 127) << 23);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x = d[n][i >> 2][i & 3];
+      if constexpr (PACK) x += dpp_f32<0x128>(x);  // row_ror:8, the other term's column
+      d[n][i >> 2][i & 3] = x * (kf * qf[n]);
+    }
+  }
+  if (tail) {
+    asm volatile("");
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (key0 + i + (i >> 2) * 12 >= limit[n]) d[n][i >> 2][i & 3] = -INFINITY;
+  }
+  auto weights = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) add[n] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float vf = ldexpf(1.f, ve_of(i) - st.eb);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float p = __builtin_amdgcn_exp2f(d[n][i >> 2][i & 3] - st.mt[n]);
+        add[n] += p;
+        w[n][i] = p * vf;
+      }
+    }
+  };
+  weights();
+  bool over = st.fresh || high - st.eb > 100;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
+    over |= big > 32768.f || add[n] > 0x1p110f;
+  }
+  if (__any(over)) {
+    // New levels: the largest x + ve of a row at 2^8.
+    asm volatile("");
+    int e1 = high;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) e1 = max(e1, __shfl_xor(e1, o, 64));
+    const int eb1 = max(st.eb, __builtin_amdgcn_readfirstlane(e1));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float mx = -INFINITY, mw = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        mx = fmaxf(mx, d[n][i >> 2][i & 3]);
+        mw = fmaxf(mw, d[n][i >> 2][i & 3] + (float)ve_of(i));
+      }
+      st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
+      st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
+      float m1 = fmaxf(st.top_w[n] - (float)eb1 - 8.f, st.top_x[n] - 100.f);
+      if (m1 == -INFINITY) m1 = 0.f;  // no key yet
+      const float keep = st.fresh ? 0.f : __builtin_amdgcn_exp2f(st.mt[n] - m1);
+      const float keep_o =
+          st.fresh ? 0.f : __builtin_amdgcn_exp2f(st.mt[n] - m1 + (float)(st.eb - eb1));
+      st.l[n] *= keep;
+#pragma unroll
+      for (int j = 0; j < DT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.acc[n][j][r] *= keep_o;
+      st.mt[n] = m1;
+    }
+    st.eb = eb1;
+    st.fresh = false;
+    weights();
+  }
+  if (__any(bad & 0x80808080u)) {  // a row that sees a NaN row becomes NaN
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool kn = byte_s(ek[i >> 2], i & 3) == kNanExp, vn = ve_of(i) == kNanExp;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        if (key0 + i + (i >> 2) * 12 < limit[n]) {
+          if (kn) add[n] = __int_as_float(0x7FC00000);
+          if (kn || vn) w[n][i] = __int_as_float(0x7FC00000);
+        }
+    }
+  }
+  uint32_t ph[NT][4], plo[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    st.l[n] += add[n];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) split2(w[n][2 * i], w[n][2 * i + 1], ph[n][i], plo[n][i]);
+  }
+  // O^T += V^T P^T.
+#pragma unroll
+  for (int j = 0; j < DT; j += 2) {
+    const f16x8 v0 = vfrag(j), v1 = vfrag(j + 1);
+    if constexpr (PACK) {
+      const bool hi = c < 8;
+      const f16x8 pb = f16x8_of(make_uint4(hi ? ph[0][0] : plo[0][0], hi ? ph[0][1] : plo[0][1],
+                                           hi ? ph[0][2] : plo[0][2], hi ? ph[0][3] : plo[0][3]));
+      st.acc[0][j] = mfma16(v0, pb, st.acc[0][j]);
+      st.acc[0][j + 1] = mfma16(v1, pb, st.acc[0][j + 1]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const f16x8 pb = f16x8_of(make_uint4(ph[n][0], ph[n][1], ph[n][2], ph[n][3]));
+        st.acc[n][j] = mfma16(v0, pb, st.acc[n][j]);
+        st.acc[n][j + 1] = mfma16(v1, pb, st.acc[n][j + 1]);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const f16x8 pb = f16x8_of(make_uint4(plo[n][0], plo[n][1], plo[n][2], plo[n][3]));
+        st.acc[n][j] = mfma16(v0, pb, st.acc[n][j]);
+        st.acc[n][j + 1] = mfma16(v1, pb, st.acc[n][j + 1]);
+      }
+    }
+  }
+}
+
+// A job's rows as a wave holds them: which ones, and the keys they see.
+template <int NT, bool PACK, bool SHARED>
+struct JobRows {
+  RowRef ref[NT];
+  uint32_t limit[NT], least, most;
+
+  __device__ __forceinline__ void init(const AttnQ8Args& a, uint32_t b, uint32_t kvh,
+                                       uint32_t row0, uint32_t nrows, uint32_t pkeys, int c) {
+    most = 0;
+    least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint32_t r = row0 + n * 16 + (PACK ? c & 7 : c);
+      ref[n] = row_ref<SHARED>(a, b, kvh, min(r, nrows - 1), pkeys);
+      if (r >= nrows) ref[n].live = false, ref[n].limit = 0;
+      limit[n] = ref[n].limit;
+      most = max(most, limit[n]);
+      if (limit[n]) least = min(least, limit[n]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+      most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+      least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+  }
+};
+
+// Byte J of the lane's eight keys as an A operand of V.
+template <int J>
+__device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride) {
+  return f16x8_of(make_uint4(pair_f16<J>(v[0], v[stride]), pair_f16<J>(v[2 * stride], v[3 * stride]),
+                             pair_f16<J>(v[4 * stride], v[5 * stride]),
+                             pair_f16<J>(v[6 * stride], v[7 * stride])));
+}
+__device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride, int j) {
+  switch (j & 3) {
+    case 0: return v_frag<0>(v, stride);
+    case 1: return v_frag<1>(v, stride);
+    case 2: return v_frag<2>(v, stride);
+    default: return v_frag<3>(v, stride);
+  }
+}
+
 // SHARED: the prefix's keys for the rows of all sequences, as partial results.
 // Otherwise a sequence's own keys; with one split (and the prefix's partial
 // results, where there are) the block writes the output itself.
@@ -363,24 +607,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
   const Q8Cache& src = SHARED ? a.pre : a.c;
   const uint32_t pkeys = a.prefix_len ? min(*a.prefix_len, a.pre.max_rows) : 0;
 
-  RowRef ref[NT];
-  uint32_t most = 0, least = 0xFFFFFFFFu;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const uint32_t r = row0 + n * 16 + (PACK ? c & 7 : c);
-    ref[n] = row_ref<SHARED>(a, b, kvh, min(r, nrows - 1), pkeys);
-    if (r >= nrows) ref[n].limit = 0;
-    most = max(most, ref[n].limit);
-    if (ref[n].limit) least = min(least, ref[n].limit);
-  }
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) {
-    most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-    least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
-  }
-  most = __builtin_amdgcn_readfirstlane(most);
-  least = __builtin_amdgcn_readfirstlane(least);
-
+  JobRows<NT, PACK, SHARED> rows;
+  rows.init(a, b, kvh, row0, nrows, pkeys, c);
+  const RowRef* ref = rows.ref;
   f16x8 qh[NT][KS], ql[PACK ? 1 : NT][KS];
   float qf[NT];
 #pragma unroll
@@ -395,20 +624,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
     }
   }
 
-  f32x4 acc[NT][DT];
-  float mt[NT], top_x[NT], top_w[NT], l[NT];
-  int eb = -126;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    mt[n] = 0.f;
-    top_x[n] = top_w[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int j = 0; j < DT; ++j) acc[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  RowsState<ROW, NT> st;
+  st.init();
 
   // The split's tiles [t0, t1), the waves' in turn.
-  const uint32_t tiles = (most + 31) / 32;
+  const uint32_t tiles = (rows.most + 31) / 32;
   const uint32_t per = (tiles + splits - 1) / splits;
   const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
   const size_t base = ((size_t)(SHARED ? 0 : b) * src.kv_heads + kvh) * src.cap;
@@ -419,159 +639,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
   Tile<ROW> cur;
   uint32_t t = t0 + wave;
   if (t < t1) load_tile<ROW>(cur, kp, vp, kep, vep, t * 32, g, c);
-  bool fresh = true;
   for (; t < t1; t += WAVES) {
     Tile<ROW> next;
     load_tile<ROW>(next, kp, vp, kep, vep, min(t + WAVES, t1 - 1) * 32, g, c);
 
-    f32x4 d[NT][2];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) d[n][hh] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const uint4 w = cur.k[hh][s >> 1];
-        const f16x8 ka = (s & 1) ? codes8_f16(w.z, w.w) : codes8_f16(w.x, w.y);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          d[n][hh] = mfma16(ka, qh[n][s], d[n][hh]);
-          if constexpr (!PACK) d[n][hh] = mfma16(ka, ql[n][s], d[n][hh]);
-        }
-      }
-    }
-    // Exponents of the lane's eight keys.
-    const bool tail = t * 32 + 32 > least;
-    const uint32_t key0 = t * 32 + 4 * g;  // + i, and + 12 + i from the fifth on
-    int ek[8], ev[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ek[i] = byte_s(cur.ke[i >> 2], i & 3);
-      ev[i] = byte_s(cur.ve[i >> 2], i & 3);
-    }
-    if (tail) {  // behind the rows' last key there may be anything
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (key0 + i + (i >> 2) * 12 >= most) ek[i] = ev[i] = -126;
-    }
-    int low = 0, high = -126;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      low = min(low, min(ek[i], ev[i]));
-      high = max(high, ev[i]);
-    }
-    const bool nans = __any(low == kNanExp);
-    // Scores, in units of ln 2.
-    float x[NT][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float kf = __int_as_float((ek[i] + 127) << 23);
-      if (nans) kf = ek[i] == kNanExp ? __int_as_float(0x7FC00000) : kf;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float s = d[n][i >> 2][i & 3];
-        if constexpr (PACK) s += dpp_f32<0x128>(s);  // row_ror:8, the other term's column
-        x[n][i] = s * (kf * qf[n]);
-        if (tail) x[n][i] = key0 + i + (i >> 2) * 12 >= ref[n].limit ? -INFINITY : x[n][i];
-      }
-    }
-    uint32_t ph[NT][4], plo[NT][4];
-    float add[NT];
-    bool redo = fresh;
-#pragma unroll 1
-    for (int round = 0; round < 2; ++round) {  // the second one's levels fit
-      if (redo) {
-        // New levels: the largest x + ve of a row at 2^8.
-        int e1 = high;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) e1 = max(e1, __shfl_xor(e1, o, 64));
-        const int eb1 = max(eb, __builtin_amdgcn_readfirstlane(e1));
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float mx = -INFINITY, mw = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            mx = fmaxf(mx, x[n][i]);
-            mw = fmaxf(mw, x[n][i] + (float)ev[i]);
-          }
-          mx = xor_max<32>(xor_max<16>(mx));
-          mw = xor_max<32>(xor_max<16>(mw));
-          top_x[n] = fmaxf(top_x[n], ceilf(mx));
-          top_w[n] = fmaxf(top_w[n], ceilf(mw));
-          float m1 = fmaxf(top_w[n] - (float)eb1 - 8.f, top_x[n] - 100.f);
-          if (m1 == -INFINITY) m1 = 0.f;  // no key yet
-          const float keep = fresh ? 0.f : __builtin_amdgcn_exp2f(mt[n] - m1);
-          const float keep_o =
-              fresh ? 0.f : __builtin_amdgcn_exp2f(mt[n] - m1 + (float)(eb - eb1));
-          l[n] *= keep;
-#pragma unroll
-          for (int j = 0; j < DT; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[n][j][r] *= keep_o;
-          mt[n] = m1;
-        }
-        eb = eb1;
-        fresh = false;
-      }
-      bool over = high - eb > 100;
-      float vf[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        vf[i] = ldexpf(1.f, ev[i] - eb);
-        if (nans) vf[i] = ev[i] == kNanExp ? __int_as_float(0x7FC00000) : vf[i];
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float w[8], big = 0.f;
-        add[n] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(x[n][i] - mt[n]);
-          add[n] += p;
-          w[i] = p * vf[i];
-          if (tail) w[i] = key0 + i + (i >> 2) * 12 >= ref[n].limit ? 0.f : w[i];
-          big = fmaxf(big, w[i]);
-        }
-        over |= big > 32768.f || add[n] > 0x1p110f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split2(w[2 * i], w[2 * i + 1], ph[n][i], plo[n][i]);
-      }
-      redo = __any(over);
-      if (!redo) break;
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) l[n] += add[n];
-    // O^T += V^T P^T.
-#pragma unroll
-    for (int j = 0; j < DT; ++j) {
-      constexpr int W = ROW / 64;
-      const int wd = j / 4;
-      uint32_t p4[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t v0 = cur.v[2 * i][W == 1 ? 0 : wd], v1 = cur.v[2 * i + 1][W == 1 ? 0 : wd];
-        switch (j & 3) {
-          case 0: p4[i] = pair_f16<0>(v0, v1); break;
-          case 1: p4[i] = pair_f16<1>(v0, v1); break;
-          case 2: p4[i] = pair_f16<2>(v0, v1); break;
-          default: p4[i] = pair_f16<3>(v0, v1); break;
-        }
-      }
-      const f16x8 va = f16x8_of(make_uint4(p4[0], p4[1], p4[2], p4[3]));
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if constexpr (PACK) {
-          const bool hi = c < 8;
-          acc[n][j] = mfma16(va, f16x8_of(make_uint4(hi ? ph[n][0] : plo[n][0], hi ? ph[n][1] : plo[n][1],
-                                                     hi ? ph[n][2] : plo[n][2], hi ? ph[n][3] : plo[n][3])),
-                             acc[n][j]);
-        } else {
-          acc[n][j] = mfma16(va, f16x8_of(make_uint4(ph[n][0], ph[n][1], ph[n][2], ph[n][3])), acc[n][j]);
-          acc[n][j] = mfma16(va, f16x8_of(make_uint4(plo[n][0], plo[n][1], plo[n][2], plo[n][3])),
-                             acc[n][j]);
-        }
-      }
-    }
+    tile_step<ROW, NT, PACK>(
+        st, qh, ql, qf, rows.limit, rows.least, rows.most, t, g, c, cur.ke, cur.ve,
+        [&](int hh, int s) {
+          const uint4 w = cur.k[hh][s >> 1];
+          return (s & 1) ? codes8_f16(w.z, w.w) : codes8_f16(w.x, w.y);
+        },
+        [&](int j) { return v_frag(&cur.v[0][j / 4], ROW / 64, j); });
     cur = next;
   }
 
@@ -584,18 +662,18 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
   __shared__ float2 sfin[RT];  // maximum and sum of a row over all its parts
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float total = xor_sum<32>(xor_sum<16>(l[n]));
+    const float total = xor_sum<32>(xor_sum<16>(st.l[n]));
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const int row = n * 16 + c;
     const bool mine = !PACK || c < 8;
-    if (g == 0 && mine) sml[wave][row] = {total == 0.f ? -INFINITY : mt[n], total};
+    if (g == 0 && mine) sml[wave][row] = {total == 0.f ? -INFINITY : st.mt[n], total};
 #pragma unroll
     for (int j = 0; j < DT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float o = acc[n][j][r];
+        float o = st.acc[n][j][r];
         if constexpr (PACK) o += dpp_f32<0x128>(o);
-        if (mine && ref[n].limit) so[wave][row][(4 * g + r) * DT + j] = ldexpf(o * inv, eb);
+        if (mine && ref[n].limit) so[wave][row][(4 * g + r) * DT + j] = ldexpf(o * inv, st.eb);
       }
   }
   __syncthreads();
@@ -641,11 +719,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
     if (x.live && fin.y != 0.f) {
       for (int w = 0; w < WAVES; ++w)
         if (sw[row][w] != 0.f) o += sw[row][w] * so[w][row][col];
-      if constexpr (!SHARED)
+      if constexpr (!SHARED) {
+        const float* q = po + row_id(a, x) * nparts * ROW + col;
+#pragma unroll 8
         for (uint32_t p = 0; p < extra; ++p) {
-          const float f = sw[row][WAVES + p];
-          if (f != 0.f) o += f * po[(row_id(a, x) * nparts + p) * ROW + col];
+          const float f = sw[row][WAVES + p], y = q[(size_t)p * ROW];
+          o += f == 0.f ? 0.f : f * y;  // an empty part's row may hold anything
         }
+      }
       o /= fin.y;
     }
     if (final) {
@@ -661,41 +742,293 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
   }
 }
 
-// Joins a row's partial results: one wave per row and head.
+// The same for jobs of 32 RW rows: the block's waves convert each stage of 64
+// keys to fp16 once, into LDS in the order of the MFMAs' operands, and every wave
+// takes its 32 rows (wave % RW) over one of the stage's two 32-key tiles (wave / RW) from there;
+// the tiles' halves are joined at the end.  The next stage's codes are on
+// their way while a stage is computed, and are converted into the other half
+// of the buffer.
+template <int ROW, int RW, bool SHARED>
+__global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, AttnQ8Plan pl) {
+  constexpr int KS = ROW / 32, DT = ROW / 16, NT = 2, U = ROW / 64, W = 2 * RW;
+  constexpr int FRAGS = 2 * KS + DT;                  // of a tile, 1 KB each
+  constexpr int NK = 4 * U, NV = 2 * U;               // conversion units of a stage
+  constexpr int KU = (NK + W - 1) / W, VU = (NV + W - 1) / W;
+  constexpr int RS = ROW + 4;
+  constexpr size_t kBuffers = (size_t)2 * 2 * FRAGS * 64;  // in uint4
+  constexpr size_t kJoin = (size_t)RW * 32 * RS / 4 + RW * 16;
+  __shared__ uint4 smem[kBuffers > kJoin ? kBuffers : kJoin];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, c = lane & 15;
+  const int rw = wave % RW, kw = wave / RW;
+  uint32_t id = blockIdx.x;
+  const uint32_t splits = SHARED ? pl.prefix_splits : pl.own_splits;
+  const uint32_t groups = SHARED ? pl.prefix_groups : pl.own_groups;
+  const uint32_t group = id % groups;
+  id /= groups;
+  const uint32_t kvh = id % a.c.kv_heads;
+  id /= a.c.kv_heads;
+  const uint32_t split = id % splits;
+  const uint32_t b = id / splits;  // 0 when SHARED
+  const uint32_t G = a.heads / a.c.kv_heads;
+  const uint32_t nrows = SHARED ? a.batch * a.rows * G : a.rows * G;
+  const Q8Cache& src = SHARED ? a.pre : a.c;
+  const uint32_t pkeys = a.prefix_len ? min(*a.prefix_len, a.pre.max_rows) : 0;
+  JobRows<NT, false, SHARED> rows;
+  rows.init(a, b, kvh, group * 32 * RW + rw * 32, nrows, pkeys, c);
+  // The block goes as far as its furthest row.
+  __shared__ uint32_t furthest[RW];
+  if (kw == 0 && lane == 0) furthest[rw] = rows.most;
+  f16x8 qh[NT][KS], ql[NT][KS];
+  float qf[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) qf[n] = load_q<ROW>(a, rows.ref[n], g, qh[n], ql[n]);
+  __syncthreads();
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < RW; ++i) most = max(most, furthest[i]);
+
+  const uint32_t tiles = (most + 31) / 32;
+  const uint32_t per = ((tiles + 1) / 2 + splits - 1) / splits * 2;  // whole stages
+  const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
+  const size_t base = ((size_t)(SHARED ? 0 : b) * src.kv_heads + kvh) * src.cap;
+  const int8_t* kp = src.k + base * ROW;
+  const int8_t* vp = src.v + base * ROW;
+  const int8_t* kep = src.ke + base;
+  const int8_t* vep = src.ve + base;
+
+  uint4 rk[KU];
+  uint32_t rv[VU][8], ke[2], ve[2];
+  auto load = [&](uint32_t t) {  // the stage of tiles t and t + 1
+#pragma unroll
+    for (int i = 0; i < KU; ++i) {
+      const int u = wave + i * W;
+      if (u < NK) {
+        const uint32_t key = min(t + u / (2 * U), t1 - 1) * 32 + u / U % 2 * 16 + c;
+        rk[i] = *reinterpret_cast<const uint4*>(kp + (size_t)key * ROW + 16 * g + u % U * 64);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VU; ++i) {
+      const int u = W - 1 - wave + i * W;
+      if (u < NV) {
+        const uint32_t key = min(t + u / U, t1 - 1) * 32 + 4 * g;
+        const int8_t* q = vp + (size_t)key * ROW + c * (ROW / 16) + u % U * 4;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          rv[i][k] = *reinterpret_cast<const uint32_t*>(q + ((k & 3) + (k >> 2) * 16) * ROW);
+      }
+    }
+    const uint32_t key = min(t + kw, t1 - 1) * 32 + 4 * g;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      ke[hh] = *reinterpret_cast<const uint32_t*>(kep + key + 16 * hh);
+      ve[hh] = *reinterpret_cast<const uint32_t*>(vep + key + 16 * hh);
+    }
+  };
+  auto store = [&](int half) {
+    uint4* to = smem + (size_t)half * 2 * FRAGS * 64 + lane;
+#pragma unroll
+    for (int i = 0; i < KU; ++i) {
+      const int u = wave + i * W;
+      if (u < NK) {
+        uint4* f = to + (u / (2 * U) * FRAGS + u / U % 2 * KS + u % U * 2) * 64;
+        f[0] = __builtin_bit_cast(uint4, codes8_f16(rk[i].x, rk[i].y));
+        f[64] = __builtin_bit_cast(uint4, codes8_f16(rk[i].z, rk[i].w));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VU; ++i) {
+      const int u = W - 1 - wave + i * W;
+      if (u < NV) {
+        uint4* f = to + (u / U * FRAGS + 2 * KS + u % U * 4) * 64;
+        f[0] = __builtin_bit_cast(uint4, v_frag<0>(rv[i], 1));
+        f[64] = __builtin_bit_cast(uint4, v_frag<1>(rv[i], 1));
+        f[128] = __builtin_bit_cast(uint4, v_frag<2>(rv[i], 1));
+        f[192] = __builtin_bit_cast(uint4, v_frag<3>(rv[i], 1));
+      }
+    }
+  };
+
+  RowsState<ROW, NT> st;
+  st.init();
+  if (t0 < t1) {
+    load(t0);
+    store(0);
+  }
+  int half = 0;
+  for (uint32_t t = t0; t < t1; t += 2) {
+    __syncthreads();
+    const uint32_t cke[2] = {ke[0], ke[1]}, cve[2] = {ve[0], ve[1]};
+    if (t + 2 < t1) load(t + 2);
+    if (t + kw < t1 && (t + kw) * 32 < rows.most) {
+      const uint4* f = smem + ((size_t)half * 2 + kw) * FRAGS * 64 + lane;
+      tile_step<ROW, NT, false>(
+          st, qh, ql, qf, rows.limit, rows.least, rows.most, t + kw, g, c, cke, cve,
+          [&](int hh, int s) { return f16x8_of(f[(hh * KS + s) * 64]); },
+          [&](int j) { return f16x8_of(f[(2 * KS + j) * 64]); });
+    }
+    half ^= 1;
+    if (t + 2 < t1) store(half);
+  }
+
+  // The second tiles' waves hand their normalised rows to the first's.
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem);
+  PartMl* sml = reinterpret_cast<PartMl*>(so + (size_t)RW * 32 * RS);
+  float m[NT], total[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    total[n] = xor_sum<32>(xor_sum<16>(st.l[n]));
+    m[n] = total[n] == 0.f ? -INFINITY : st.mt[n];
+    const float inv = total[n] == 0.f ? 0.f : 1.f / total[n];
+#pragma unroll
+    for (int j = 0; j < DT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st.acc[n][j][r] = ldexpf(st.acc[n][j][r] * inv, st.eb);
+    const int row = rw * 32 + n * 16 + c;
+    if (kw == 1) {
+      if (g == 0) sml[row] = {m[n], total[n]};
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < DT; j += 4)
+          *reinterpret_cast<float4*>(so + (size_t)row * RS + (4 * g + r) * DT + j) =
+              make_float4(st.acc[n][j][r], st.acc[n][j + 1][r], st.acc[n][j + 2][r],
+                          st.acc[n][j + 3][r]);
+    }
+  }
+  __syncthreads();
+  if (kw == 1) return;
+  const bool final = !SHARED && pl.own_splits == 1;
+  const uint32_t extra = final ? pl.prefix_splits : 0;
+  PartMl* ml = reinterpret_cast<PartMl*>(a.ws);
+  float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
+  const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
+  const uint32_t at = SHARED ? split : pl.prefix_splits + split;
+  const uint32_t hd = a.c.head_dim;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const RowRef x = rows.ref[n];
+    const uint32_t r0 = group * 32 * RW + rw * 32 + n * 16 + c;
+    if (r0 >= nrows || (!x.live && !final)) continue;
+    const int row = rw * 32 + n * 16 + c;
+    const size_t part = row_id(a, x) * nparts;
+    const PartMl y = sml[row];
+    float top = fmaxf(m[n], y.m);
+    for (uint32_t e = 0; e < extra && x.live; ++e) top = fmaxf(top, ml[part + e].m);
+    const float f0 = total[n] == 0.f ? 0.f : total[n] * __builtin_amdgcn_exp2f(m[n] - top);
+    const float f1 = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - top);
+    float sum = f0 + f1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < DT; j += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(so + (size_t)row * RS + (4 * g + r) * DT + j);
+        const float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float o = f0 == 0.f ? 0.f : f0 * st.acc[n][j + i][r];
+          if (f1 != 0.f) o += f1 * w[i];
+          st.acc[n][j + i][r] = o;
+        }
+      }
+    for (uint32_t e = 0; e < extra && x.live; ++e) {
+      const PartMl z = ml[part + e];
+      if (z.l == 0.f) continue;
+      const float f = z.l * __builtin_amdgcn_exp2f(z.m - top);
+      sum += f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < DT; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(po + (part + e) * ROW + (4 * g + r) * DT + j);
+          st.acc[n][j][r] += f * v.x;
+          st.acc[n][j + 1][r] += f * v.y;
+          st.acc[n][j + 2][r] += f * v.z;
+          st.acc[n][j + 3][r] += f * v.w;
+        }
+    }
+    const bool some = x.live && sum != 0.f;
+    const float inv = some ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < DT; j += 4) {
+        const float4 v = some ? make_float4(st.acc[n][j][r] * inv, st.acc[n][j + 1][r] * inv,
+                                            st.acc[n][j + 2][r] * inv, st.acc[n][j + 3][r] * inv)
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint32_t col = (4 * g + r) * DT + j;
+        if (!final) {
+          *reinterpret_cast<float4*>(po + (part + at) * ROW + col) = v;
+        } else {
+          float* out = a.out + x.bt * a.out_stride + (size_t)x.head * hd + col;
+          if (a.out_vec && col + 4 <= hd) {
+            *reinterpret_cast<float4*>(out) = v;
+          } else {
+            if (col < hd) out[0] = v.x;
+            if (col + 1 < hd) out[1] = v.y;
+            if (col + 2 < hd) out[2] = v.z;
+            if (col + 3 < hd) out[3] = v.w;
+          }
+        }
+      }
+    if (g == 0) {
+      if (!final)
+        ml[part + at] = {some ? top : -INFINITY, some ? sum : 0.f};
+      else if (a.lse)
+        a.lse[row_id(a, x)] = some ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+  }
+}
+
+// Joins a row's partial results: one block per row and head, a wave takes
+// every fourth part.
 template <int ROW>
 __global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan pl) {
-  const uint64_t id = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= (uint64_t)a.batch * a.rows * a.heads) return;
-  const int lane = threadIdx.x & 63;
-  const uint64_t bt = id / a.heads;
-  const uint32_t b = (uint32_t)(bt / a.rows), t = (uint32_t)(bt % a.rows);
-  float* out = a.out + bt * a.out_stride + (id % a.heads) * a.c.head_dim;
-  const uint32_t n = pl.prefix_splits + pl.own_splits;
-  const PartMl* ml = reinterpret_cast<const PartMl*>(a.ws) + id * n;
-  const float* po = reinterpret_cast<const float*>(static_cast<const char*>(a.ws) + pl.rows_offset) +
-                    id * n * ROW;
-  const bool live = t < step_rows(a.counts, b, a.rows);
-  float m = -INFINITY, total = 0.f, o[ROW / 64] = {};
-  if (live) {
-    for (uint32_t p = 0; p < n; ++p) m = fmaxf(m, ml[p].m);
-    for (uint32_t p = 0; p < n; ++p) {
-      const PartMl y = ml[p];
-      if (y.l == 0.f) continue;
-      const float f = y.l * __builtin_amdgcn_exp2f(y.m - m);
-      total += f;
+  constexpr int C = ROW / 64;
+  const uint32_t id = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t bt = id / a.heads;
+  const uint32_t b = bt / a.rows, t = bt % a.rows;
+  float* out = a.out + (size_t)bt * a.out_stride + (size_t)(id % a.heads) * a.c.head_dim;
+  const int n = pl.prefix_splits + pl.own_splits;  // at most two a lane
+  const PartMl* ml = reinterpret_cast<const PartMl*>(a.ws) + (size_t)id * n;
+  const float* po =
+      reinterpret_cast<const float*>(static_cast<const char*>(a.ws) + pl.rows_offset) +
+      (size_t)id * n * ROW + lane;
+  __shared__ float part[4][ROW];
+  float m = -INFINITY, total = 0.f, o[C] = {};
+  if (t < step_rows(a.counts, b, a.rows)) {
+    PartMl y[2];
 #pragma unroll
-      for (int i = 0; i < ROW / 64; ++i) {
-        const uint32_t col = lane + 64 * i;
-        if (col < a.c.head_dim) o[i] += f * po[(size_t)p * ROW + col];
+    for (int i = 0; i < 2; ++i)
+      y[i] = lane + 64 * i < n ? ml[lane + 64 * i] : PartMl{-INFINITY, 0.f};
+    m = wave_max(fmaxf(y[0].m, y[1].m));
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      f[i] = y[i].l == 0.f ? 0.f : y[i].l * __builtin_amdgcn_exp2f(y[i].m - m);
+    total = wave_sum(f[0] + f[1]);
+#pragma unroll 8
+    for (int p = wave; p < n; p += 4) {
+      const float w = __shfl(p < 64 ? f[0] : f[1], p & 63, 64);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const float x = po[(size_t)p * ROW + 64 * i];
+        o[i] += w == 0.f ? 0.f : w * x;  // an empty part's row may hold anything
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < ROW / 64; ++i) {
-    const uint32_t col = lane + 64 * i;
-    if (col < a.c.head_dim) out[col] = total == 0.f ? 0.f : o[i] / total;
-  }
-  if (lane == 0 && a.lse)
+  for (int i = 0; i < C; ++i) part[wave][lane + 64 * i] = o[i];
+  __syncthreads();
+  const uint32_t col = threadIdx.x;
+  if (col < a.c.head_dim)
+    out[col] = total == 0.f
+                   ? 0.f
+                   : (((part[0][col] + part[1][col]) + part[2][col]) + part[3][col]) / total;
+  if (threadIdx.x == 0 && a.lse)
     a.lse[id] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.6931471805599453f;
 }
 
@@ -735,8 +1068,18 @@ hipError_t launch_cache_read_q8(const Q8Cache& c, float* k, float* v, uint32_t b
 
 namespace {
 
-// Rows of a job: 8 in packed columns, else 16 or 32.
-uint32_t rows_per_job(uint64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+// Rows of a job: 8 in packed columns, 16, or 32, 64 and 128 by way of LDS.
+uint32_t rows_per_job(uint64_t rows) {
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+}
+
+// Splits of `tiles` 32-key tiles among blocks, for `jobs` jobs of rt rows.
+uint32_t key_splits(uint64_t jobs, uint64_t tiles, uint32_t rt) {
+  const uint64_t want = rt <= 16 ? 1024 : rt <= 64 ? 512 : 256;
+  const uint64_t least = rt <= 16 ? 16 : 4;  // tiles that are worth a block
+  return (uint32_t)std::max<uint64_t>(
+      1, std::min<uint64_t>({kAttnMaxSplits, tiles / least, div_up(want, jobs)}));
+}
 
 AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   AttnQ8Plan p{};
@@ -744,18 +1087,13 @@ AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   const uint64_t own = a.rows * G, all = own * a.batch;
   p.own_rt = rows_per_job(own);
   p.own_groups = (uint32_t)div_up(own, p.own_rt);
-  const uint64_t jobs = (uint64_t)a.batch * a.c.kv_heads * p.own_groups;
-  const uint64_t want = 1024, tiles = div_up(a.max_len, 32);
-  auto splits = [&](uint64_t jobs, uint64_t tiles) {
-    const uint64_t by_work = tiles / 16;  // four tiles a wave at least
-    return (uint32_t)std::max<uint64_t>(
-        1, std::min<uint64_t>({kAttnMaxSplits, by_work, div_up(want, jobs)}));
-  };
-  p.own_splits = splits(jobs, tiles);
+  p.own_splits = key_splits((uint64_t)a.batch * a.c.kv_heads * p.own_groups,
+                            div_up(a.max_len, 32), p.own_rt);
   if (prefix) {
     p.prefix_rt = rows_per_job(all);
     p.prefix_groups = (uint32_t)div_up(all, p.prefix_rt);
-    p.prefix_splits = splits((uint64_t)a.c.kv_heads * p.prefix_groups, div_up(a.pre.max_rows, 32));
+    p.prefix_splits = key_splits((uint64_t)a.c.kv_heads * p.prefix_groups,
+                                 div_up(a.pre.max_rows, 32), p.prefix_rt);
   }
   const uint64_t parts = p.prefix_splits + (p.own_splits > 1 ? p.own_splits : 0);
   const uint64_t ids = (uint64_t)a.batch * a.rows * a.heads;
@@ -769,12 +1107,13 @@ void launch_parts(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
   const uint32_t rt = SHARED ? p.prefix_rt : p.own_rt;
   const dim3 grid(SHARED ? p.prefix_groups * a.c.kv_heads * p.prefix_splits
                          : a.batch * p.own_splits * a.c.kv_heads * p.own_groups);
-  if (rt == 8)
-    hipLaunchKernelGGL((k_attn_q8<ROW, 1, true, 4, SHARED>), grid, dim3(256), 0, s, a, p);
-  else if (rt == 16)
-    hipLaunchKernelGGL((k_attn_q8<ROW, 1, false, 4, SHARED>), grid, dim3(256), 0, s, a, p);
-  else
-    hipLaunchKernelGGL((k_attn_q8<ROW, 2, false, 4, SHARED>), grid, dim3(256), 0, s, a, p);
+  auto* f = rt == 8    ? k_attn_q8<ROW, 1, true, 4, SHARED>
+            : rt == 16 ? k_attn_q8<ROW, 1, false, 4, SHARED>
+            : rt == 32 ? k_attn_q8_rows<ROW, 1, SHARED>
+            : rt == 64 ? k_attn_q8_rows<ROW, 2, SHARED>
+                       : k_attn_q8_rows<ROW, 4, SHARED>;
+  const uint32_t threads = rt <= 16 ? 256 : rt * 4;
+  hipLaunchKernelGGL(f, grid, dim3(threads), 0, s, a, p);
 }
 
 template <int ROW>
@@ -782,9 +1121,8 @@ hipError_t launch_attn(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) 
   if (p.prefix_splits) launch_parts<ROW, true>(a, p, s);
   launch_parts<ROW, false>(a, p, s);
   if (p.own_splits > 1)
-    hipLaunchKernelGGL((k_attn_q8_join<ROW>),
-                       dim3((uint32_t)div_up((uint64_t)a.batch * a.rows * a.heads, 4)), dim3(256),
-                       0, s, a, p);
+    hipLaunchKernelGGL((k_attn_q8_join<ROW>), dim3(a.batch * a.rows * a.heads), dim3(256), 0, s, a,
+                       p);
   return hipGetLastError();
 }
 
@@ -797,6 +1135,7 @@ size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix) {
 hipError_t launch_attn_q8(AttnQ8Args a, hipStream_t s) {
   const AttnQ8Plan p = attn_q8_plan(a, a.prefix_len != nullptr);
   a.q_vec = vec4(a.q, a.q_stride, a.c.head_dim);
+  a.out_vec = vec4(a.out, a.out_stride, a.c.head_dim);
   return a.c.row == 128 ? launch_attn<128>(a, p, s) : launch_attn<64>(a, p, s);
 }
 
