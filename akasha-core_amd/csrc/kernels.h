@@ -573,11 +573,14 @@ struct AttnQ8Args {
   uint32_t batch, rows, heads, q_stride, out_stride, max_len;
   float scale;
   void* ws;
-  bool q_vec, out_vec;  // rows of q and out as float4 (set by the launch)
+  // Set by the launch:
+  float scale_log2;     // scale * log2(e)
+  bool q_vec, out_vec;  // rows of q and out can be read as float4
 };
 // How an attention call is dealt to blocks, from its sizes alone.
 constexpr uint32_t kAttnMaxSplits = 64;
 struct AttnQ8Plan {
+  uint32_t G;                                        // query heads of a kv head
   uint32_t own_rt, own_groups, own_splits;           // rows a job, jobs, splits of the keys
   uint32_t prefix_rt, prefix_groups, prefix_splits;  // splits 0: no prefix
   size_t rows_offset, bytes;  // the workspace: maxima and sums, then rows

@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
@@ -201,16 +202,23 @@ __device__ __forceinline__ uint32_t pair_f16(uint32_t a, uint32_t b) {
 }
 
 // Two floats of at most 2^15 as hi + lo fp16 pairs: hi truncated to 11
-// bits, lo the next 11 (their sum within 2^-21, or 2^-24 below fp16's normal
-// range).
+// bits, lo the rest rounded to 11 (together within 2^-22, or 2^-25 below fp16's
+// normal range).
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const float ha = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u);
-  const float hb = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(ha, hb));
-  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - ha, b - hb));
+  const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+  const h2 l = {(_Float16)fmaf((float)h[0], -1.f, a), (_Float16)fmaf((float)h[1], -1.f, b)};
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
 }
 
-__device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+// Four exponents with 127 added to each byte (kNanExp: 255), and one of
+// them as 2^e (kNanExp: infinity).
+__device__ __forceinline__ uint32_t biased(uint32_t w) {
+  return ((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) ^ (w & 0x80808080u);
+}
+__device__ __forceinline__ float biased_power(uint32_t w, int i) {
+  return __uint_as_float((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7F800000u);
+}
 
 // What one 32-key tile's lane loads.
 template <int ROW>
@@ -257,76 +265,153 @@ struct RowRef {
   bool live;       // it is the step's (otherwise it sees no key)
 };
 
-// Row r of a job's rows (SHARED: of every sequence), G query heads each.
+// A job's place, and what its rows see.
 template <bool SHARED>
-__device__ __forceinline__ RowRef row_ref(const AttnQ8Args& a, uint32_t b, uint32_t kvh,
-                                          uint32_t r, uint32_t prefix_keys) {
-  const uint32_t G = a.heads / a.c.kv_heads;
-  RowRef x;
-  uint32_t t = r / G;
-  x.head = kvh * G + r % G;
-  if constexpr (SHARED) {
-    b = t / a.rows;
-    t -= b * a.rows;
-  }
-  x.live = b < a.batch && t < step_rows(a.counts, b, a.rows);
-  x.limit = 0;
-  if (x.live)
-    x.limit = SHARED ? prefix_keys
-                     : (uint32_t)min<uint64_t>((uint64_t)a.pos[b] + t + 1, a.c.max_rows);
-  x.bt = (uint64_t)b * a.rows + t;
-  return x;
-}
+struct Job {
+  uint32_t b, kvh, group, split, splits, nrows, G;
+  uint32_t live_rows;  // of the sequence; SHARED: unused
+  uint32_t pos;
+  uint32_t keys;       // the prefix's
 
-// q of one row as MFMA B operands, hi and lo, scaled by scale log2(e) and by
-// 2^-e to a largest magnitude in [2^13, 2^14); returns 2^e, NaN for a row
-// with a NaN or an infinity.
+  __device__ __forceinline__ void init(const AttnQ8Args& a, const AttnQ8Plan& pl) {
+    uint32_t id = blockIdx.x;
+    const uint32_t groups = SHARED ? pl.prefix_groups : pl.own_groups;
+    splits = SHARED ? pl.prefix_splits : pl.own_splits;
+    G = pl.G;
+    group = 0;
+    if (groups > 1) {
+      group = id % groups;
+      id /= groups;
+    }
+    kvh = id % a.c.kv_heads;
+    id /= a.c.kv_heads;
+    split = 0;
+    if (SHARED) {
+      split = id;
+    } else if (splits > 1) {
+      split = id % splits;
+      id /= splits;
+    }
+    b = SHARED ? 0 : id;
+    nrows = (SHARED ? a.batch : 1) * a.rows * G;
+    if constexpr (SHARED) {
+      keys = min(*a.prefix_len, a.pre.max_rows);
+    } else {
+      live_rows = step_rows(a.counts, b, a.rows);
+      pos = a.pos[b];
+    }
+  }
+  __device__ __forceinline__ uint32_t sees(const AttnQ8Args& a, uint32_t t) const {
+    return (uint32_t)min<uint64_t>((uint64_t)pos + t + 1, a.c.max_rows);
+  }
+  // Row r of the job's kv head, G query heads each (SHARED: of every sequence).
+  __device__ __forceinline__ RowRef row(const AttnQ8Args& a, uint32_t r) const {
+    RowRef x;
+    x.live = r < nrows;
+    r = min(r, nrows - 1);
+    uint32_t t = r, h = 0, s = b;
+    if (G > 1) {
+      t = r / G;
+      h = r - t * G;
+    }
+    if constexpr (SHARED) {
+      s = t;
+      if (a.rows > 1) s = t / a.rows;
+      t -= s * a.rows;
+      x.live = x.live && t < step_rows(a.counts, s, a.rows);
+      x.limit = x.live ? keys : 0;
+    } else {
+      x.live = x.live && t < live_rows;
+      x.limit = x.live ? sees(a, t) : 0;
+    }
+    x.head = kvh * G + h;
+    x.bt = (uint64_t)s * a.rows + t;
+    return x;
+  }
+  // Keys that any (most) and every live row (least) of rows row0 .. + n - 1
+  // sees.
+  __device__ __forceinline__ void span(const AttnQ8Args& a, uint32_t row0, uint32_t n,
+                                       uint32_t& least, uint32_t& most) const {
+    if constexpr (SHARED) {
+      least = most = keys;
+    } else {
+      uint32_t first = row0, last = min(row0 + n, nrows) - 1;
+      if (G > 1) {
+        first /= G;
+        last /= G;
+      }
+      const bool some = row0 < nrows && first < live_rows;
+      least = some ? sees(a, first) : 0xFFFFFFFFu;
+      most = some ? sees(a, min(last, live_rows - 1)) : 0;
+    }
+  }
+};
+
+// q of one row, as the lane's columns of the MFMA steps.
 template <int ROW>
-__device__ __forceinline__ float load_q(const AttnQ8Args& a, const RowRef& r, int g, f16x8* hi,
-                                        f16x8* lo) {
-  constexpr int KS = ROW / 32;
-  const float* q = a.q + r.bt * a.q_stride + (size_t)r.head * a.c.head_dim;
-  const float cs = (float)((double)a.scale * 1.4426950408889634);
-  const int hd = (int)a.c.head_dim;
-  float x[KS][8];
-  float top = 0.f, sum = 0.f;
+struct RawQ {
+  float x[ROW / 32][8];
+
+  __device__ __forceinline__ void load(const AttnQ8Args& a, const RowRef& r, int g) {
+    const float* q = a.q + r.bt * a.q_stride + (size_t)r.head * a.c.head_dim;
+    const int hd = (int)a.c.head_dim;
+    if (a.q_vec) {  // head_dim is a multiple of 4
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    const int d0 = (s >> 1) * 64 + 16 * g + 8 * (s & 1);
-    if (a.q_vec && d0 + 8 <= hd && r.limit) {
-      const float4 u = *reinterpret_cast<const float4*>(q + d0);
-      const float4 w = *reinterpret_cast<const float4*>(q + d0 + 4);
-      x[s][0] = u.x, x[s][1] = u.y, x[s][2] = u.z, x[s][3] = u.w;
-      x[s][4] = w.x, x[s][5] = w.y, x[s][6] = w.z, x[s][7] = w.w;
+      for (int s = 0; s < ROW / 32; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const int d = (s >> 1) * 64 + 16 * g + 8 * (s & 1) + i;
+          const float4 u = *reinterpret_cast<const float4*>(q + min(d, hd - 4));
+          const bool in = d < hd;
+          x[s][i] = in ? u.x : 0.f;
+          x[s][i + 1] = in ? u.y : 0.f;
+          x[s][i + 2] = in ? u.z : 0.f;
+          x[s][i + 3] = in ? u.w : 0.f;
+        }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[s][i] = r.limit && d0 + i < hd ? q[d0 + i] : 0.f;
-    }
+      for (int s = 0; s < ROW / 32; ++s)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[s][i] *= cs;
-      top = fmaxf(top, fabsf(x[s][i]));
-      sum += x[s][i] * 0.f;  // NaN where anything is not finite
+        for (int i = 0; i < 8; ++i) {
+          const int d = (s >> 1) * 64 + 16 * g + 8 * (s & 1) + i;
+          const float u = q[min(d, hd - 1)];
+          x[s][i] = d < hd ? u : 0.f;
+        }
     }
   }
-  top = xor_max<32>(xor_max<16>(top));
-  sum = xor_sum<32>(xor_sum<16>(sum));
-  // top = 1.m 2^(E - 127); times 2^(140 - E) it is 1.m 2^13 (E at least 15, so
-  // that 2^e stays a normal number's inverse; smaller rows keep small terms).
-  const int E = max(15, (int)(__float_as_uint(top) >> 23));
-  const float s1 = ldexpf(1.f, 140 - E), back = ldexpf(1.f, E - 140);
-  const bool ok = sum == 0.f;
+
+  // As B operands, hi and lo, scaled by scale log2(e) and by 2^-e to a largest
+  // magnitude in [2^13, 2^14); returns 2^e, NaN for a row with a NaN or an
+  // infinity.
+  __device__ __forceinline__ float operands(const AttnQ8Args& a, f16x8* hi, f16x8* lo) {
+    float top = 0.f, sum = 0.f;
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    uint32_t h[4], l[4];
+    for (int s = 0; s < ROW / 32; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      split2(ok ? x[s][2 * i] * s1 : 0.f, ok ? x[s][2 * i + 1] * s1 : 0.f, h[i], l[i]);
-    hi[s] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
-    lo[s] = f16x8_of(make_uint4(l[0], l[1], l[2], l[3]));
+      for (int i = 0; i < 8; ++i) {
+        x[s][i] *= a.scale_log2;
+        top = fmaxf(top, fabsf(x[s][i]));
+        sum += x[s][i] * 0.f;  // NaN where anything is not finite
+      }
+    top = xor_max<32>(xor_max<16>(top));
+    sum = xor_sum<32>(xor_sum<16>(sum));
+    // top = 1.m 2^(E - 127); times 2^(140 - E) it is 1.m 2^13 (E at least 15, so
+    // that both powers are normal numbers; smaller rows keep small terms).
+    const int E = max(15, (int)(__float_as_uint(top) >> 23));
+    const float s1 = ldexpf(1.f, 140 - E), back = ldexpf(1.f, E - 140);
+    const bool ok = sum == 0.f;
+#pragma unroll
+    for (int s = 0; s < ROW / 32; ++s) {
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        split2(ok ? x[s][2 * i] * s1 : 0.f, ok ? x[s][2 * i + 1] * s1 : 0.f, h[i], l[i]);
+      hi[s] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
+      lo[s] = f16x8_of(make_uint4(l[0], l[1], l[2], l[3]));
+    }
+    return ok ? back : __int_as_float(0x7FC00000);
   }
-  return ok ? back : __int_as_float(0x7FC00000);
-}
+};
 
 // Partial results of a row: maximum (log2), sum and normalised weighted row
 // of each part; the prefix's splits first, then the own rows'.
@@ -346,7 +431,7 @@ struct RowsState {
   bool fresh;
 
   __device__ __forceinline__ void init() {
-    eb = -126;
+    eb = 0;
     fresh = true;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -360,14 +445,15 @@ struct RowsState {
 };
 
 // One tile of 32 keys: kfrag(hh, s) and vfrag(j) give K's and V's A operands,
-// ke / ve the lane's exponents.  limit: keys a row sees; least and most of
-// all rows' (of those that see any) decide whether the tile needs the mask.
-template <int ROW, int NT, bool PACK, class KF, class VF>
+// kscale(hh) and vscale(hh) the powers of two of the lane's four keys of half hh (infinity
+// for a NaN row; finite behind the last key that any row sees), nan whether the tile has a
+// NaN row.  limit: keys a row sees; a tile past the least of them needs the mask.
+template <int ROW, int NT, bool PACK, class KF, class VF, class KS4, class VS4>
 __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*qh)[ROW / 32],
                                           const f16x8 (*ql)[ROW / 32], const float* qf,
-                                          const uint32_t* limit, uint32_t least, uint32_t most,
-                                          uint32_t tile, int g, int c, const uint32_t* ke,
-                                          const uint32_t* ve, KF kfrag, VF vfrag) {
+                                          const uint32_t* limit, uint32_t least, uint32_t tile,
+                                          int g, int c, bool nan, KF kfrag, VF vfrag, KS4 kscale,
+                                          VS4 vscale) {
   constexpr int KS = ROW / 32, DT = ROW / 16;
   f32x4 d[NT][2];
 #pragma unroll
@@ -390,65 +476,51 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   }
   // The rare cases are branches of their own that patch what the common path
   // made (the empty asm keeps them branches).
-  const uint32_t key0 = tile * 32 + 4 * g;  // + i, and + 12 + i from the fifth on
-  uint32_t ek[2] = {ke[0], ke[1]}, ev[2] = {ve[0], ve[1]};
-  const bool tail = tile * 32 + 32 > least;
-  if (tail) {  // behind the rows' last key the exponents may be anything
-    asm volatile("");
+  const uint32_t key0 = tile * 32 + 4 * g;  // + r, and + 16 + r in the second half
+  if constexpr (PACK) {
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int left = (int)min(most, key0 + 16 * hh + 4) - (int)(key0 + 16 * hh);
-      const uint32_t keep = left <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * left);
-      ek[hh] = (ek[hh] & keep) | (0x82828282u & ~keep);
-      ev[hh] = (ev[hh] & keep) | (0x82828282u & ~keep);
-    }
+    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)  // row_ror:8, the other term's column
+        d[0][hh][r] += dpp_f32<0x128>(d[0][hh][r]);
   }
-  auto ve_of = [&](int i) { return byte_s(ev[i >> 2], i & 3); };
-  int high = -126;
-  uint32_t bad = 0;  // a byte 0x80 is kNanExp
-#pragma unroll
-  for (int i = 0; i < 8; ++i) high = max(high, ve_of(i));
-#pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    const uint32_t x = ek[hh] ^ 0x80808080u, y = ev[hh] ^ 0x80808080u;
-    bad |= (x - 0x01010101u) & ~x;
-    bad |= (y - 0x01010101u) & ~y;
-  }
-  float w[NT][8], add[NT];  // scores (in units of ln 2 once scaled), then weights
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float kf = __int_as_float((byte_s(ek[i >> 2], i & 3) + 127) << 23);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float x = d[n][i >> 2][i & 3];
-      if constexpr (PACK) x += dpp_f32<0x128>(x);  // row_ror:8, the other term's column
-      d[n][i >> 2][i & 3] = x * (kf * qf[n]);
-    }
-  }
-  if (tail) {
-    asm volatile("");
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (key0 + i + (i >> 2) * 12 >= limit[n]) d[n][i >> 2][i & 3] = -INFINITY;
-  }
-  auto weights = [&]() {
+  auto sees = [&](int n, int i) { return key0 + (i & 3) + (i >> 2) * 16 < limit[n]; };
+  float w[NT][8], add[NT];
+  auto weights = [&](auto masked) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) add[n] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float vf = ldexpf(1.f, ve_of(i) - st.eb);
+    for (int hh = 0; hh < 2; ++hh) {
+      const f32x4 kf = kscale(hh);
+      f32x4 vf = vscale(hh);
+      if (st.eb != 0) {
+        asm volatile("");
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float p = __builtin_amdgcn_exp2f(d[n][i >> 2][i & 3] - st.mt[n]);
-        add[n] += p;
-        w[n][i] = p * vf;
+        for (int r = 0; r < 4; ++r) vf[r] = fminf(ldexpf(vf[r], -st.eb), 0x1p120f);
       }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float p = __builtin_amdgcn_exp2f(fmaf(d[n][hh][r], kf[r] * qf[n], -st.mt[n]));
+          float x = p * vf[r];
+          if constexpr (decltype(masked)::value) {
+            const bool in = sees(n, 4 * hh + r);
+            p = in ? p : 0.f;
+            x = in ? x : 0.f;
+          }
+          add[n] += p;
+          w[n][4 * hh + r] = x;
+        }
     }
   };
-  weights();
-  bool over = st.fresh || high - st.eb > 100;
+  if (tile * 32 + 32 > least) {
+    asm volatile("");
+    weights(std::true_type{});
+  } else {
+    weights(std::false_type{});
+  }
+  bool over = st.fresh;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float big = 0.f;
@@ -456,20 +528,35 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
     over |= big > 32768.f || add[n] > 0x1p110f;
   }
-  if (__any(over)) {
-    // New levels: the largest x + ve of a row at 2^8.
+  if (st.eb != 0) {  // (0x1p120 stands for more)
     asm volatile("");
-    int e1 = high;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) e1 = max(e1, __shfl_xor(e1, o, 64));
-    const int eb1 = max(st.eb, __builtin_amdgcn_readfirstlane(e1));
+    for (int i = 0; i < 8; ++i) over |= ldexpf(vscale(i >> 2)[i & 3], -st.eb) > 0x1p119f;
+  }
+  if (__any(over)) {
+    // New levels: the largest x + ve of a row at 2^8.  eb is 0 unless the
+    // values' scales are far from 1.
+    asm volatile("");
+    float e1 = -126.f, lv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = vscale(i >> 2)[i & 3];
+      lv[i] = v < INFINITY ? (float)((int)(__float_as_uint(v) >> 23) - 127) : 0.f;
+      e1 = fmaxf(e1, v < INFINITY ? lv[i] : -126.f);
+    }
+    e1 = xor_max<32>(xor_max<16>(e1));  // alike in the columns' lanes
+    const int high = (int)__builtin_amdgcn_readfirstlane((int)e1);
+    int eb1 = st.eb;
+    if (st.fresh ? high > 60 || high < -60 : st.eb == 0 ? high > 60 : high > st.eb) eb1 = high;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        mx = fmaxf(mx, d[n][i >> 2][i & 3]);
-        mw = fmaxf(mw, d[n][i >> 2][i & 3] + (float)ve_of(i));
+        const float x = d[n][i >> 2][i & 3] * (kscale(i >> 2)[i & 3] * qf[n]);
+        const bool in = sees(n, i);
+        mx = fmaxf(mx, in ? x : -INFINITY);
+        mw = fmaxf(mw, in ? x + lv[i] : -INFINITY);
       }
       st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
@@ -487,19 +574,18 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     }
     st.eb = eb1;
     st.fresh = false;
-    weights();
+    weights(std::true_type{});
   }
-  if (__any(bad & 0x80808080u)) {  // a row that sees a NaN row becomes NaN
+  if (nan) {  // a row that sees a NaN row becomes NaN, the others do not
     asm volatile("");
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool kn = byte_s(ek[i >> 2], i & 3) == kNanExp, vn = ve_of(i) == kNanExp;
+      const bool kn = !(kscale(i >> 2)[i & 3] < INFINITY), vn = !(vscale(i >> 2)[i & 3] < INFINITY);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        if (key0 + i + (i >> 2) * 12 < limit[n]) {
-          if (kn) add[n] = __int_as_float(0x7FC00000);
-          if (kn || vn) w[n][i] = __int_as_float(0x7FC00000);
-        }
+      for (int n = 0; n < NT; ++n) {
+        if (kn && sees(n, i)) add[n] = __int_as_float(0x7FC00000);
+        if ((kn || vn) && sees(n, i)) w[n][i] = __int_as_float(0x7FC00000);
+      }
     }
   }
   uint32_t ph[NT][4], plo[NT][4];
@@ -536,35 +622,6 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   }
 }
 
-// A job's rows as a wave holds them: which ones, and the keys they see.
-template <int NT, bool PACK, bool SHARED>
-struct JobRows {
-  RowRef ref[NT];
-  uint32_t limit[NT], least, most;
-
-  __device__ __forceinline__ void init(const AttnQ8Args& a, uint32_t b, uint32_t kvh,
-                                       uint32_t row0, uint32_t nrows, uint32_t pkeys, int c) {
-    most = 0;
-    least = 0xFFFFFFFFu;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint32_t r = row0 + n * 16 + (PACK ? c & 7 : c);
-      ref[n] = row_ref<SHARED>(a, b, kvh, min(r, nrows - 1), pkeys);
-      if (r >= nrows) ref[n].live = false, ref[n].limit = 0;
-      limit[n] = ref[n].limit;
-      most = max(most, limit[n]);
-      if (limit[n]) least = min(least, limit[n]);
-    }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
-      least = min(least, (uint32_t)__shfl_xor((int)least, o, 64));
-    }
-    most = __builtin_amdgcn_readfirstlane(most);
-    least = __builtin_amdgcn_readfirstlane(least);
-  }
-};
-
 // Byte J of the lane's eight keys as an A operand of V.
 template <int J>
 __device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride) {
@@ -584,141 +641,160 @@ __device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride, int j) {
 // SHARED: the prefix's keys for the rows of all sequences, as partial results.
 // Otherwise a sequence's own keys; with one split (and the prefix's partial
 // results, where there are) the block writes the output itself.
-template <int ROW, int NT, bool PACK, int WAVES, bool SHARED>
+template <int ROW, bool PACK, int WAVES, bool SHARED>
 __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan pl) {
-  constexpr int KS = ROW / 32;           // MFMA steps of a score
-  constexpr int DT = ROW / 16;           // MFMAs of 16 output columns
-  constexpr int RT = PACK ? 8 : 16 * NT; // rows of a job
-  static_assert(!PACK || NT == 1, "one packed tile");
+  constexpr int KS = ROW / 32;       // MFMA steps of a score
+  constexpr int DT = ROW / 16;       // MFMAs of 16 output columns
+  constexpr int RT = PACK ? 8 : 16;  // rows of a job
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c = lane & 15;
-  uint32_t id = blockIdx.x;
-  const uint32_t splits = SHARED ? pl.prefix_splits : pl.own_splits;
-  const uint32_t groups = SHARED ? pl.prefix_groups : pl.own_groups;
-  const uint32_t group = id % groups;
-  id /= groups;
-  const uint32_t kvh = id % a.c.kv_heads;
-  id /= a.c.kv_heads;
-  const uint32_t split = id % splits;
-  const uint32_t b = id / splits;  // 0 when SHARED
-  const uint32_t G = a.heads / a.c.kv_heads;
-  const uint32_t nrows = SHARED ? a.batch * a.rows * G : a.rows * G;
-  const uint32_t row0 = group * RT;
+  Job<SHARED> job;
+  job.init(a, pl);
+  const uint32_t row0 = job.group * RT;
   const Q8Cache& src = SHARED ? a.pre : a.c;
-  const uint32_t pkeys = a.prefix_len ? min(*a.prefix_len, a.pre.max_rows) : 0;
-
-  JobRows<NT, PACK, SHARED> rows;
-  rows.init(a, b, kvh, row0, nrows, pkeys, c);
-  const RowRef* ref = rows.ref;
-  f16x8 qh[NT][KS], ql[PACK ? 1 : NT][KS];
-  float qf[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    if constexpr (PACK) {
-      f16x8 lo[KS];
-      qf[n] = load_q<ROW>(a, ref[n], g, qh[n], lo);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) qh[n][s] = c < 8 ? qh[n][s] : lo[s];
-    } else {
-      qf[n] = load_q<ROW>(a, ref[n], g, qh[n], ql[n]);
-    }
-  }
-
-  RowsState<ROW, NT> st;
-  st.init();
-
-  // The split's tiles [t0, t1), the waves' in turn.
-  const uint32_t tiles = (rows.most + 31) / 32;
-  const uint32_t per = (tiles + splits - 1) / splits;
-  const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
-  const size_t base = ((size_t)(SHARED ? 0 : b) * src.kv_heads + kvh) * src.cap;
+  const size_t base = ((size_t)job.b * src.kv_heads + job.kvh) * src.cap;
   const int8_t* kp = src.k + base * ROW;
   const int8_t* vp = src.v + base * ROW;
   const int8_t* kep = src.ke + base;
   const int8_t* vep = src.ve + base;
+
+  // q, and with one split the first tile (inside the cache wherever the rows
+  // end), are under way before the lengths have arrived.
+  const RowRef ref = job.row(a, row0 + (PACK ? c & 7 : c));
+  RawQ<ROW> raw;
+  raw.load(a, ref, g);
   Tile<ROW> cur;
+  const bool early = job.splits == 1;
+  if (early)
+    load_tile<ROW>(cur, kp, vp, kep, vep, min((uint32_t)wave * 32, src.cap - 32), g, c);
+  // The split's tiles [t0, t1), the waves' in turn.
+  uint32_t least, most;
+  job.span(a, row0, RT, least, most);
+  const uint32_t tiles = (most + 31) / 32;
+  const uint32_t per = early ? tiles : (tiles + job.splits - 1) / job.splits;
+  const uint32_t t0 = min(tiles, job.split * per), t1 = min(tiles, t0 + per);
   uint32_t t = t0 + wave;
-  if (t < t1) load_tile<ROW>(cur, kp, vp, kep, vep, t * 32, g, c);
+  if (!early && t < t1) load_tile<ROW>(cur, kp, vp, kep, vep, t * 32, g, c);
+
+  f16x8 qh[1][KS], ql[1][KS];
+  const float qf = raw.operands(a, qh[0], ql[0]);
+  if constexpr (PACK) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qh[0][s] = c < 8 ? qh[0][s] : ql[0][s];
+  }
+  RowsState<ROW, 1> st;
+  st.init();
   for (; t < t1; t += WAVES) {
     Tile<ROW> next;
     load_tile<ROW>(next, kp, vp, kep, vep, min(t + WAVES, t1 - 1) * 32, g, c);
-
-    tile_step<ROW, NT, PACK>(
-        st, qh, ql, qf, rows.limit, rows.least, rows.most, t, g, c, cur.ke, cur.ve,
+    if (t * 32 + 32 > most) {  // behind the rows' last key the exponents may be anything
+      asm volatile("");
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const uint32_t key = t * 32 + 16 * hh + 4 * g;
+        const int left = (int)min(most, key + 4) - (int)key;
+        const uint32_t keep = left <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * left);
+        cur.ke[hh] = (cur.ke[hh] & keep) | (0x82828282u & ~keep);
+        cur.ve[hh] = (cur.ve[hh] & keep) | (0x82828282u & ~keep);
+      }
+    }
+    const uint32_t bk[2] = {biased(cur.ke[0]), biased(cur.ke[1])};
+    const uint32_t bv[2] = {biased(cur.ve[0]), biased(cur.ve[1])};
+    uint32_t nan = 0;  // a byte of 255
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh)
+      nan |= ((~bk[hh] - 0x01010101u) & bk[hh]) | ((~bv[hh] - 0x01010101u) & bv[hh]);
+    tile_step<ROW, 1, PACK>(
+        st, qh, ql, &qf, &ref.limit, least, t, g, c, __any(nan & 0x80808080u),
         [&](int hh, int s) {
           const uint4 w = cur.k[hh][s >> 1];
           return (s & 1) ? codes8_f16(w.z, w.w) : codes8_f16(w.x, w.y);
         },
-        [&](int j) { return v_frag(&cur.v[0][j / 4], ROW / 64, j); });
+        [&](int j) { return v_frag(&cur.v[0][j / 4], ROW / 64, j); },
+        [&](int hh) {
+          return f32x4{biased_power(bk[hh], 0), biased_power(bk[hh], 1), biased_power(bk[hh], 2),
+                       biased_power(bk[hh], 3)};
+        },
+        [&](int hh) {
+          return f32x4{biased_power(bv[hh], 0), biased_power(bv[hh], 1), biased_power(bv[hh], 2),
+                       biased_power(bv[hh], 3)};
+        });
     cur = next;
   }
 
-  // Join the waves: each one's row normalised, weighted by its sum.
-  constexpr int RS = ROW + 4;
-  constexpr int MAXP = kAttnMaxSplits;
+  // Join the waves: each one's row normalised, weighted by its sum; and with
+  // them the prefix's parts, 64 WAVES / RT lanes to a row.
+  constexpr int RS = ROW + 4, L = 64 * WAVES / RT;
+  constexpr int MAXP = SHARED ? 0 : kAttnMaxSplits, NP = (MAXP + L - 1) / L;
   __shared__ float so[WAVES][RT][RS];
   __shared__ PartMl sml[WAVES][RT];
-  __shared__ float sw[RT][WAVES + (SHARED ? 0 : MAXP)];
+  __shared__ float sw[RT][WAVES + MAXP];
   __shared__ float2 sfin[RT];  // maximum and sum of a row over all its parts
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const float total = xor_sum<32>(xor_sum<16>(st.l[n]));
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    const int row = n * 16 + c;
-    const bool mine = !PACK || c < 8;
-    if (g == 0 && mine) sml[wave][row] = {total == 0.f ? -INFINITY : st.mt[n], total};
-#pragma unroll
-    for (int j = 0; j < DT; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float o = st.acc[n][j][r];
-        if constexpr (PACK) o += dpp_f32<0x128>(o);
-        if (mine && ref[n].limit) so[wave][row][(4 * g + r) * DT + j] = ldexpf(o * inv, st.eb);
-      }
-  }
-  __syncthreads();
   const bool final = !SHARED && pl.own_splits == 1;
   const uint32_t extra = final ? pl.prefix_splits : 0;
-  const PartMl* ml = reinterpret_cast<const PartMl*>(a.ws);
+  PartMl* ml = reinterpret_cast<PartMl*>(a.ws);
   float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
   const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
-  if (threadIdx.x < RT) {
-    const int row = threadIdx.x;
-    const RowRef x = row_ref<SHARED>(a, b, kvh, min(row0 + row, nrows - 1), pkeys);
-    float m = -INFINITY;
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, sml[w][row].m);
-    const bool live = row0 + row < nrows && x.live;
-    if (live)
-      for (uint32_t e = 0; e < extra; ++e) m = fmaxf(m, ml[row_id(a, x) * nparts + e].m);
-    float total = 0.f;
-    for (int w = 0; w < WAVES; ++w) {
-      const PartMl y = sml[w][row];
-      const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
-      sw[row][w] = f;
-      total += f;
-    }
-    if constexpr (!SHARED)
-      for (uint32_t e = 0; live && e < extra; ++e) {
-        const PartMl y = ml[row_id(a, x) * nparts + e];
-        const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
-        sw[row][WAVES + e] = f;
-        total += f;
+  const int jrow = threadIdx.x / L, jl = threadIdx.x % L;
+  const RowRef jref = job.row(a, row0 + jrow);
+  PartMl pre[NP > 0 ? NP : 1];
+#pragma unroll
+  for (int i = 0; i < NP; ++i)
+    pre[i] = jref.live && jl + i * L < (int)extra ? ml[row_id(a, jref) * nparts + jl + i * L]
+                                                  : PartMl{-INFINITY, 0.f};
+  const float total = xor_sum<32>(xor_sum<16>(st.l[0]));
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const bool mine = !PACK || c < 8;
+  if (g == 0 && mine) sml[wave][c] = {total == 0.f ? -INFINITY : st.mt[0], total};
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < DT; j += 4) {
+      float o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = st.acc[0][j + i][r];
+        if constexpr (PACK) o[i] += dpp_f32<0x128>(o[i]);
+        o[i] = ldexpf(o[i] * inv, st.eb);
       }
-    sfin[row] = make_float2(m, total);
+      if (mine && ref.live)
+        *reinterpret_cast<float4*>(&so[wave][c][(4 * g + r) * DT + j]) =
+            make_float4(o[0], o[1], o[2], o[3]);
+    }
+  __syncthreads();
+  {
+    const PartMl y = jl < WAVES ? sml[jl][jrow] : PartMl{-INFINITY, 0.f};
+    float m = y.m;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) m = fmaxf(m, pre[i].m);
+    m = group_max<L>(m);
+    const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
+    float sum = f;
+    float z[NP > 0 ? NP : 1];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      z[i] = pre[i].l == 0.f ? 0.f : pre[i].l * __builtin_amdgcn_exp2f(pre[i].m - m);
+      sum += z[i];
+    }
+    sum = group_sum<L>(sum);
+    const float part = sum == 0.f ? 0.f : 1.f / sum;
+    if (jl < WAVES) sw[jrow][jl] = f * part;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (jl + i * L < (int)extra) sw[jrow][WAVES + jl + i * L] = z[i] * part;
+    if (jl == 0) sfin[jrow] = make_float2(m, sum);
   }
   __syncthreads();
   const uint32_t hd = a.c.head_dim;
-  const uint32_t rows_here = min((uint32_t)RT, nrows - row0);
-  const uint32_t at = SHARED ? split : pl.prefix_splits + split;
+  const uint32_t rows_here = min((uint32_t)RT, job.nrows - row0);
+  const uint32_t at = SHARED ? job.split : pl.prefix_splits + job.split;
   for (uint32_t e = threadIdx.x; e < rows_here * ROW; e += 64 * WAVES) {
     const uint32_t row = e / ROW, col = e % ROW;
     if (col >= hd) continue;
-    const RowRef x = row_ref<SHARED>(a, b, kvh, row0 + row, pkeys);
+    const RowRef x = job.row(a, row0 + row);
     const float2 fin = sfin[row];
     float o = 0.f;
     if (x.live && fin.y != 0.f) {
-      for (int w = 0; w < WAVES; ++w)
-        if (sw[row][w] != 0.f) o += sw[row][w] * so[w][row][col];
       if constexpr (!SHARED) {
         const float* q = po + row_id(a, x) * nparts * ROW + col;
 #pragma unroll 8
@@ -727,7 +803,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
           o += f == 0.f ? 0.f : f * y;  // an empty part's row may hold anything
         }
       }
-      o /= fin.y;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float f = sw[row][w];
+        o += f == 0.f ? 0.f : f * so[w][row][col];
+      }
     }
     if (final) {
       a.out[x.bt * a.out_stride + (size_t)x.head * hd + col] = x.live ? o : 0.f;
@@ -736,8 +816,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
             x.live && fin.y != 0.f ? (fin.x + log2f(fin.y)) * 0.6931471805599453f : -INFINITY;
     } else if (x.live) {
       po[(row_id(a, x) * nparts + at) * ROW + col] = o;
-      if (col == 0)
-        const_cast<PartMl*>(ml)[row_id(a, x) * nparts + at] = {fin.y == 0.f ? -INFINITY : fin.x, fin.y};
+      if (col == 0) ml[row_id(a, x) * nparts + at] = {fin.y == 0.f ? -INFINITY : fin.x, fin.y};
     }
   }
 }
@@ -758,47 +837,44 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   constexpr size_t kBuffers = (size_t)2 * 2 * FRAGS * 64;  // in uint4
   constexpr size_t kJoin = (size_t)RW * 32 * RS / 4 + RW * 16;
   __shared__ uint4 smem[kBuffers > kJoin ? kBuffers : kJoin];
+  __shared__ __attribute__((aligned(16))) float scales[2][2][64];  // 2^e of a stage's keys, K's and V's
+  __shared__ uint32_t nans[2][2];         // the NaN rows of its tiles
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int g = lane >> 4, c = lane & 15;
   const int rw = wave % RW, kw = wave / RW;
-  uint32_t id = blockIdx.x;
-  const uint32_t splits = SHARED ? pl.prefix_splits : pl.own_splits;
-  const uint32_t groups = SHARED ? pl.prefix_groups : pl.own_groups;
-  const uint32_t group = id % groups;
-  id /= groups;
-  const uint32_t kvh = id % a.c.kv_heads;
-  id /= a.c.kv_heads;
-  const uint32_t split = id % splits;
-  const uint32_t b = id / splits;  // 0 when SHARED
-  const uint32_t G = a.heads / a.c.kv_heads;
-  const uint32_t nrows = SHARED ? a.batch * a.rows * G : a.rows * G;
+  Job<SHARED> job;
+  job.init(a, pl);
   const Q8Cache& src = SHARED ? a.pre : a.c;
-  const uint32_t pkeys = a.prefix_len ? min(*a.prefix_len, a.pre.max_rows) : 0;
-  JobRows<NT, false, SHARED> rows;
-  rows.init(a, b, kvh, group * 32 * RW + rw * 32, nrows, pkeys, c);
-  // The block goes as far as its furthest row.
-  __shared__ uint32_t furthest[RW];
-  if (kw == 0 && lane == 0) furthest[rw] = rows.most;
+  const uint32_t row0 = job.group * 32 * RW + rw * 32;
+  RowRef ref[NT];
+  uint32_t limit[NT];
   f16x8 qh[NT][KS], ql[NT][KS];
   float qf[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) qf[n] = load_q<ROW>(a, rows.ref[n], g, qh[n], ql[n]);
-  __syncthreads();
-  uint32_t most = 0;
-#pragma unroll
-  for (int i = 0; i < RW; ++i) most = max(most, furthest[i]);
+  for (int n = 0; n < NT; ++n) {
+    ref[n] = job.row(a, row0 + n * 16 + c);
+    limit[n] = ref[n].limit;
+    RawQ<ROW> raw;
+    raw.load(a, ref[n], g);
+    qf[n] = raw.operands(a, qh[n], ql[n]);
+  }
+  // The wave's rows, and as far as the block's furthest one.
+  uint32_t least, mine, unused, most;
+  job.span(a, row0, 32, least, mine);
+  job.span(a, job.group * 32 * RW, 32 * RW, unused, most);
 
   const uint32_t tiles = (most + 31) / 32;
-  const uint32_t per = ((tiles + 1) / 2 + splits - 1) / splits * 2;  // whole stages
-  const uint32_t t0 = min(tiles, split * per), t1 = min(tiles, t0 + per);
-  const size_t base = ((size_t)(SHARED ? 0 : b) * src.kv_heads + kvh) * src.cap;
+  const uint32_t per = ((tiles + 1) / 2 + job.splits - 1) / job.splits * 2;  // whole stages
+  const uint32_t t0 = min(tiles, job.split * per), t1 = min(tiles, t0 + per);
+  const size_t base = ((size_t)job.b * src.kv_heads + job.kvh) * src.cap;
   const int8_t* kp = src.k + base * ROW;
   const int8_t* vp = src.v + base * ROW;
   const int8_t* kep = src.ke + base;
   const int8_t* vep = src.ve + base;
 
   uint4 rk[KU];
-  uint32_t rv[VU][8], ke[2], ve[2];
+  uint32_t rv[VU][8];
+  int re[2] = {0, 0};  // exponents of key `lane` of the stage, the last wave's
   auto load = [&](uint32_t t) {  // the stage of tiles t and t + 1
 #pragma unroll
     for (int i = 0; i < KU; ++i) {
@@ -819,11 +895,11 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
           rv[i][k] = *reinterpret_cast<const uint32_t*>(q + ((k & 3) + (k >> 2) * 16) * ROW);
       }
     }
-    const uint32_t key = min(t + kw, t1 - 1) * 32 + 4 * g;
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      ke[hh] = *reinterpret_cast<const uint32_t*>(kep + key + 16 * hh);
-      ve[hh] = *reinterpret_cast<const uint32_t*>(vep + key + 16 * hh);
+    if (wave == W - 1) {
+      const uint32_t key = min(t + lane / 32, t1 - 1) * 32 + lane % 32;
+      const bool in = key < most;  // behind that there may be anything
+      re[0] = in ? kep[key] : -126;
+      re[1] = in ? vep[key] : -126;
     }
   };
   auto store = [&](int half) {
@@ -848,6 +924,12 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
         f[192] = __builtin_bit_cast(uint4, v_frag<3>(rv[i], 1));
       }
     }
+    if (wave == W - 1) {
+      scales[half][0][lane] = __uint_as_float((uint32_t)(re[0] + 127) << 23 & 0x7F800000u);
+      scales[half][1][lane] = __uint_as_float((uint32_t)(re[1] + 127) << 23 & 0x7F800000u);
+      const uint64_t nan = __ballot(re[0] == kNanExp || re[1] == kNanExp);
+      if (lane < 2) nans[half][lane] = (uint32_t)(nan >> (32 * lane));
+    }
   };
 
   RowsState<ROW, NT> st;
@@ -859,14 +941,17 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   int half = 0;
   for (uint32_t t = t0; t < t1; t += 2) {
     __syncthreads();
-    const uint32_t cke[2] = {ke[0], ke[1]}, cve[2] = {ve[0], ve[1]};
     if (t + 2 < t1) load(t + 2);
-    if (t + kw < t1 && (t + kw) * 32 < rows.most) {
+    if (t + kw < t1 && (t + kw) * 32 < mine) {
       const uint4* f = smem + ((size_t)half * 2 + kw) * FRAGS * 64 + lane;
+      const float* sk = &scales[half][0][32 * kw + 4 * g];
       tile_step<ROW, NT, false>(
-          st, qh, ql, qf, rows.limit, rows.least, rows.most, t + kw, g, c, cke, cve,
+          st, qh, ql, qf, limit, least, t + kw, g, c,
+          __builtin_amdgcn_readfirstlane(nans[half][kw]) != 0,
           [&](int hh, int s) { return f16x8_of(f[(hh * KS + s) * 64]); },
-          [&](int j) { return f16x8_of(f[(2 * KS + j) * 64]); });
+          [&](int j) { return f16x8_of(f[(2 * KS + j) * 64]); },
+          [&](int hh) { return *reinterpret_cast<const f32x4*>(sk + 16 * hh); },
+          [&](int hh) { return *reinterpret_cast<const f32x4*>(sk + 64 + 16 * hh); });
     }
     half ^= 1;
     if (t + 2 < t1) store(half);
@@ -905,13 +990,12 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   PartMl* ml = reinterpret_cast<PartMl*>(a.ws);
   float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
   const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
-  const uint32_t at = SHARED ? split : pl.prefix_splits + split;
+  const uint32_t at = SHARED ? job.split : pl.prefix_splits + job.split;
   const uint32_t hd = a.c.head_dim;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const RowRef x = rows.ref[n];
-    const uint32_t r0 = group * 32 * RW + rw * 32 + n * 16 + c;
-    if (r0 >= nrows || (!x.live && !final)) continue;
+    const RowRef x = ref[n];
+    if (row0 + n * 16 + c >= job.nrows || (!x.live && !final)) continue;
     const int row = rw * 32 + n * 16 + c;
     const size_t part = row_id(a, x) * nparts;
     const PartMl y = sml[row];
@@ -919,7 +1003,14 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     for (uint32_t e = 0; e < extra && x.live; ++e) top = fmaxf(top, ml[part + e].m);
     const float f0 = total[n] == 0.f ? 0.f : total[n] * __builtin_amdgcn_exp2f(m[n] - top);
     const float f1 = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - top);
+    auto weight_of = [&](const PartMl& z) {
+      return z.l == 0.f ? 0.f : z.l * __builtin_amdgcn_exp2f(z.m - top);
+    };
     float sum = f0 + f1;
+    for (uint32_t e = 0; e < extra && x.live; ++e) sum += weight_of(ml[part + e]);
+    const bool some = x.live && sum != 0.f;
+    const float inv = some ? 1.f / sum : 0.f;
+    const float n0 = f0 * inv, n1 = f1 * inv;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -928,16 +1019,14 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
         const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float o = f0 == 0.f ? 0.f : f0 * st.acc[n][j + i][r];
-          if (f1 != 0.f) o += f1 * w[i];
+          float o = n0 == 0.f ? 0.f : n0 * st.acc[n][j + i][r];
+          if (n1 != 0.f) o += n1 * w[i];
           st.acc[n][j + i][r] = o;
         }
       }
     for (uint32_t e = 0; e < extra && x.live; ++e) {
-      const PartMl z = ml[part + e];
-      if (z.l == 0.f) continue;
-      const float f = z.l * __builtin_amdgcn_exp2f(z.m - top);
-      sum += f;
+      const float f = weight_of(ml[part + e]) * inv;
+      if (f == 0.f) continue;  // an empty part's row may hold anything
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -949,22 +1038,20 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
           st.acc[n][j + 3][r] += f * v.w;
         }
     }
-    const bool some = x.live && sum != 0.f;
-    const float inv = some ? 1.f / sum : 0.f;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int j = 0; j < DT; j += 4) {
-        const float4 v = some ? make_float4(st.acc[n][j][r] * inv, st.acc[n][j + 1][r] * inv,
-                                            st.acc[n][j + 2][r] * inv, st.acc[n][j + 3][r] * inv)
+        const float4 v = some ? make_float4(st.acc[n][j][r], st.acc[n][j + 1][r],
+                                            st.acc[n][j + 2][r], st.acc[n][j + 3][r])
                               : make_float4(0.f, 0.f, 0.f, 0.f);
         const uint32_t col = (4 * g + r) * DT + j;
         if (!final) {
           *reinterpret_cast<float4*>(po + (part + at) * ROW + col) = v;
         } else {
           float* out = a.out + x.bt * a.out_stride + (size_t)x.head * hd + col;
-          if (a.out_vec && col + 4 <= hd) {
-            *reinterpret_cast<float4*>(out) = v;
+          if (a.out_vec) {
+            if (col < hd) *reinterpret_cast<float4*>(out) = v;
           } else {
             if (col < hd) out[0] = v.x;
             if (col + 1 < hd) out[1] = v.y;
@@ -1010,6 +1097,9 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan p
     for (int i = 0; i < 2; ++i)
       f[i] = y[i].l == 0.f ? 0.f : y[i].l * __builtin_amdgcn_exp2f(y[i].m - m);
     total = wave_sum(f[0] + f[1]);
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    f[0] *= inv;
+    f[1] *= inv;
 #pragma unroll 8
     for (int p = wave; p < n; p += 4) {
       const float w = __shfl(p < 64 ? f[0] : f[1], p & 63, 64);
@@ -1025,9 +1115,7 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan p
   __syncthreads();
   const uint32_t col = threadIdx.x;
   if (col < a.c.head_dim)
-    out[col] = total == 0.f
-                   ? 0.f
-                   : (((part[0][col] + part[1][col]) + part[2][col]) + part[3][col]) / total;
+    out[col] = ((part[0][col] + part[1][col]) + part[2][col]) + part[3][col];
   if (threadIdx.x == 0 && a.lse)
     a.lse[id] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.6931471805599453f;
 }
@@ -1084,6 +1172,7 @@ uint32_t key_splits(uint64_t jobs, uint64_t tiles, uint32_t rt) {
 AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   AttnQ8Plan p{};
   const uint64_t G = a.heads / a.c.kv_heads;
+  p.G = (uint32_t)G;
   const uint64_t own = a.rows * G, all = own * a.batch;
   p.own_rt = rows_per_job(own);
   p.own_groups = (uint32_t)div_up(own, p.own_rt);
@@ -1107,8 +1196,8 @@ void launch_parts(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
   const uint32_t rt = SHARED ? p.prefix_rt : p.own_rt;
   const dim3 grid(SHARED ? p.prefix_groups * a.c.kv_heads * p.prefix_splits
                          : a.batch * p.own_splits * a.c.kv_heads * p.own_groups);
-  auto* f = rt == 8    ? k_attn_q8<ROW, 1, true, 4, SHARED>
-            : rt == 16 ? k_attn_q8<ROW, 1, false, 4, SHARED>
+  auto* f = rt == 8    ? k_attn_q8<ROW, true, 4, SHARED>
+            : rt == 16 ? k_attn_q8<ROW, false, 4, SHARED>
             : rt == 32 ? k_attn_q8_rows<ROW, 1, SHARED>
             : rt == 64 ? k_attn_q8_rows<ROW, 2, SHARED>
                        : k_attn_q8_rows<ROW, 4, SHARED>;
@@ -1134,6 +1223,7 @@ size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix) {
 
 hipError_t launch_attn_q8(AttnQ8Args a, hipStream_t s) {
   const AttnQ8Plan p = attn_q8_plan(a, a.prefix_len != nullptr);
+  a.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
   a.q_vec = vec4(a.q, a.q_stride, a.c.head_dim);
   a.out_vec = vec4(a.out, a.out_stride, a.c.head_dim);
   return a.c.row == 128 ? launch_attn<128>(a, p, s) : launch_attn<64>(a, p, s);
