@@ -211,14 +211,13 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = __builtin_bit_cast(uint32_t, l);
 }
 
-// Four exponents with 127 added to each byte (kNanExp: 255), and one of
-// them as 2^e (kNanExp: infinity).
-__device__ __forceinline__ uint32_t biased(uint32_t w) {
-  return ((w & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) ^ (w & 0x80808080u);
+__device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4 exps_of(uint32_t w) {
+  return i32x4{byte_s(w, 0), byte_s(w, 1), byte_s(w, 2), byte_s(w, 3)};
 }
-__device__ __forceinline__ float biased_power(uint32_t w, int i) {
-  return __uint_as_float((i < 3 ? w << (23 - 8 * i) : w >> 1) & 0x7F800000u);
-}
+// K exponents from here on are applied next to q's (2^29 codes times more may leave f32).
+constexpr int kBigExp = 90;
 
 // What one 32-key tile's lane loads.
 template <int ROW>
@@ -229,15 +228,21 @@ struct Tile {
 };
 
 template <int ROW>
-__device__ __forceinline__ void load_tile(Tile<ROW>& t, const int8_t* k, const int8_t* v,
-                                          const int8_t* ke, const int8_t* ve, uint32_t key0,
-                                          int g, int c) {
+__device__ __forceinline__ void load_k(Tile<ROW>& t, const int8_t* k, const int8_t* ke,
+                                       const int8_t* ve, uint32_t key0, int g, int c) {
   const int8_t* kp = k + (size_t)(key0 + c) * ROW + 16 * g;
 #pragma unroll
-  for (int hh = 0; hh < 2; ++hh)
+  for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
     for (int u = 0; u < ROW / 64; ++u)
       t.k[hh][u] = *reinterpret_cast<const uint4*>(kp + hh * 16 * ROW + u * 64);
+    t.ke[hh] = *reinterpret_cast<const uint32_t*>(ke + key0 + 16 * hh + 4 * g);
+    t.ve[hh] = *reinterpret_cast<const uint32_t*>(ve + key0 + 16 * hh + 4 * g);
+  }
+}
+template <int ROW>
+__device__ __forceinline__ void load_v(Tile<ROW>& t, const int8_t* v, uint32_t key0, int g,
+                                       int c) {
   const int8_t* vp = v + (size_t)(key0 + 4 * g) * ROW + c * (ROW / 16);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -249,11 +254,6 @@ __device__ __forceinline__ void load_tile(Tile<ROW>& t, const int8_t* k, const i
       t.v[i][0] = w.x;
       t.v[i][1] = w.y;
     }
-  }
-#pragma unroll
-  for (int hh = 0; hh < 2; ++hh) {
-    t.ke[hh] = *reinterpret_cast<const uint32_t*>(ke + key0 + 16 * hh + 4 * g);
-    t.ve[hh] = *reinterpret_cast<const uint32_t*>(ve + key0 + 16 * hh + 4 * g);
   }
 }
 
@@ -445,15 +445,16 @@ struct RowsState {
 };
 
 // One tile of 32 keys: kfrag(hh, s) and vfrag(j) give K's and V's A operands,
-// kscale(hh) and vscale(hh) the powers of two of the lane's four keys of half hh (infinity
-// for a NaN row; finite behind the last key that any row sees), nan whether the tile has a
-// NaN row.  limit: keys a row sees; a tile past the least of them needs the mask.
-template <int ROW, int NT, bool PACK, class KF, class VF, class KS4, class VS4>
+// kexp(hh) and vexp(hh) the exponents of the lane's four keys of half hh (any number
+// in range behind the last key that any row sees), odd whether the tile has a NaN
+// row or a K exponent of kBigExp.  limit: keys a row sees; a tile past the least
+// of them needs the mask.  k_used() is called once K's operands are spent.
+template <int ROW, int NT, bool PACK, class KF, class VF, class KE, class VE, class HK>
 __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*qh)[ROW / 32],
                                           const f16x8 (*ql)[ROW / 32], const float* qf,
                                           const uint32_t* limit, uint32_t least, uint32_t tile,
-                                          int g, int c, bool nan, KF kfrag, VF vfrag, KS4 kscale,
-                                          VS4 vscale) {
+                                          int g, int c, bool odd, KF kfrag, VF vfrag, KE kexp,
+                                          VE vexp, HK k_used) {
   constexpr int KS = ROW / 32, DT = ROW / 16;
   f32x4 d[NT][2];
 #pragma unroll
@@ -474,6 +475,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       }
     }
   }
+  k_used();
   // The rare cases are branches of their own that patch what the common path
   // made (the empty asm keeps them branches).
   const uint32_t key0 = tile * 32 + 4 * g;  // + r, and + 16 + r in the second half
@@ -485,67 +487,72 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
         d[0][hh][r] += dpp_f32<0x128>(d[0][hh][r]);
   }
   auto sees = [&](int n, int i) { return key0 + (i & 3) + (i >> 2) * 16 < limit[n]; };
+  float qe[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) qe[n] = qf[n];
+  int plain = 1;  // 0: K's exponents are applied already
+  if (odd) {
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = kexp(i >> 2)[i & 3];
+      const float f = e == kNanExp ? __int_as_float(0x7FC00000) : ldexpf(1.f, e);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) d[n][i >> 2][i & 3] *= f * qf[n];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) qe[n] = 1.f;
+    plain = 0;
+  }
   float w[NT][8], add[NT];
   auto weights = [&](auto masked) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) add[n] = 0.f;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
-      const f32x4 kf = kscale(hh);
-      f32x4 vf = vscale(hh);
+      const i32x4 ke = kexp(hh) * plain;
+      i32x4 ve = vexp(hh);
       if (st.eb != 0) {
         asm volatile("");
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vf[r] = fminf(ldexpf(vf[r], -st.eb), 0x1p120f);
+        ve -= st.eb;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          float p = __builtin_amdgcn_exp2f(fmaf(d[n][hh][r], kf[r] * qf[n], -st.mt[n]));
-          float x = p * vf[r];
-          if constexpr (decltype(masked)::value) {
-            const bool in = sees(n, 4 * hh + r);
-            p = in ? p : 0.f;
-            x = in ? x : 0.f;
-          }
+          float p =
+              __builtin_amdgcn_exp2f(fmaf(ldexpf(d[n][hh][r], ke[r]), qe[n], -st.mt[n]));
+          if constexpr (decltype(masked)::value) p = sees(n, 4 * hh + r) ? p : 0.f;
           add[n] += p;
-          w[n][4 * hh + r] = x;
+          w[n][4 * hh + r] = ldexpf(p, ve[r]);
         }
     }
   };
-  if (tile * 32 + 32 > least) {
-    asm volatile("");
-    weights(std::true_type{});
-  } else {
-    weights(std::false_type{});
-  }
   bool over = st.fresh;
+  if (!st.fresh) {
+    if (tile * 32 + 32 > least) {
+      asm volatile("");
+      weights(std::true_type{});
+    } else {
+      weights(std::false_type{});
+    }
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float big = 0.f;
+    for (int n = 0; n < NT; ++n) {
+      float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
-    over |= big > 32768.f || add[n] > 0x1p110f;
-  }
-  if (st.eb != 0) {  // (0x1p120 stands for more)
-    asm volatile("");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) over |= ldexpf(vscale(i >> 2)[i & 3], -st.eb) > 0x1p119f;
+      for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
+      over |= big > 32768.f || add[n] > 0x1p110f;
+    }
   }
   if (__any(over)) {
     // New levels: the largest x + ve of a row at 2^8.  eb is 0 unless the
     // values' scales are far from 1.
     asm volatile("");
-    float e1 = -126.f, lv[8];
+    int high = -126;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float v = vscale(i >> 2)[i & 3];
-      lv[i] = v < INFINITY ? (float)((int)(__float_as_uint(v) >> 23) - 127) : 0.f;
-      e1 = fmaxf(e1, v < INFINITY ? lv[i] : -126.f);
-    }
-    e1 = xor_max<32>(xor_max<16>(e1));  // alike in the columns' lanes
-    const int high = (int)__builtin_amdgcn_readfirstlane((int)e1);
+    for (int i = 0; i < 8; ++i) high = max(high, vexp(i >> 2)[i & 3]);
+    high = max(high, __shfl_xor(high, 16, 64));  // the columns' lanes hold the same keys
+    high = __builtin_amdgcn_readfirstlane(max(high, __shfl_xor(high, 32, 64)));
     int eb1 = st.eb;
     if (st.fresh ? high > 60 || high < -60 : st.eb == 0 ? high > 60 : high > st.eb) eb1 = high;
 #pragma unroll
@@ -553,70 +560,74 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = d[n][i >> 2][i & 3] * (kscale(i >> 2)[i & 3] * qf[n]);
+        const float x = ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] * plain) * qe[n];
         const bool in = sees(n, i);
         mx = fmaxf(mx, in ? x : -INFINITY);
-        mw = fmaxf(mw, in ? x + lv[i] : -INFINITY);
+        mw = fmaxf(mw, in ? x + (float)vexp(i >> 2)[i & 3] : -INFINITY);
       }
       st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
       float m1 = fmaxf(st.top_w[n] - (float)eb1 - 8.f, st.top_x[n] - 100.f);
       if (m1 == -INFINITY) m1 = 0.f;  // no key yet
-      const float keep = st.fresh ? 0.f : __builtin_amdgcn_exp2f(st.mt[n] - m1);
-      const float keep_o =
-          st.fresh ? 0.f : __builtin_amdgcn_exp2f(st.mt[n] - m1 + (float)(st.eb - eb1));
-      st.l[n] *= keep;
+      if (!st.fresh) {
+        st.l[n] *= __builtin_amdgcn_exp2f(st.mt[n] - m1);
+        const float keep = __builtin_amdgcn_exp2f(st.mt[n] - m1 + (float)(st.eb - eb1));
 #pragma unroll
-      for (int j = 0; j < DT; ++j)
+        for (int j = 0; j < DT; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st.acc[n][j][r] *= keep_o;
+          for (int r = 0; r < 4; ++r) st.acc[n][j][r] *= keep;
+      }
       st.mt[n] = m1;
     }
     st.eb = eb1;
     st.fresh = false;
     weights(std::true_type{});
   }
-  if (nan) {  // a row that sees a NaN row becomes NaN, the others do not
+  if (odd) {  // a row that sees a NaN row of V becomes NaN (K's made its scores NaN)
     asm volatile("");
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool kn = !(kscale(i >> 2)[i & 3] < INFINITY), vn = !(vscale(i >> 2)[i & 3] < INFINITY);
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (kn && sees(n, i)) add[n] = __int_as_float(0x7FC00000);
-        if ((kn || vn) && sees(n, i)) w[n][i] = __int_as_float(0x7FC00000);
-      }
-    }
+      for (int n = 0; n < NT; ++n)
+        if (vexp(i >> 2)[i & 3] == kNanExp && sees(n, i)) w[n][i] = __int_as_float(0x7FC00000);
   }
-  uint32_t ph[NT][4], plo[NT][4];
+  // The weights as B operands: hi and lo, or (PACK) the one of the lane's column.
+  f16x8 ph[NT], pl[PACK ? 1 : NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    uint32_t h[4], o[4];
     st.l[n] += add[n];
+    if constexpr (PACK) {
+      const uint32_t cut = c < 8 ? 0u : 0xFFFFE000u;  // hi's bits
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split2(w[n][2 * i], w[n][2 * i + 1], ph[n][i], plo[n][i]);
+      for (int i = 0; i < 4; ++i) {
+        const float x = w[n][2 * i], y = w[n][2 * i + 1];
+        h[i] = __builtin_bit_cast(
+            uint32_t,
+            __builtin_amdgcn_cvt_pkrtz(x - __uint_as_float(__float_as_uint(x) & cut),
+                                       y - __uint_as_float(__float_as_uint(y) & cut)));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split2(w[n][2 * i], w[n][2 * i + 1], h[i], o[i]);
+      pl[n] = f16x8_of(make_uint4(o[0], o[1], o[2], o[3]));
+    }
+    ph[n] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
   }
   // O^T += V^T P^T.
 #pragma unroll
   for (int j = 0; j < DT; j += 2) {
     const f16x8 v0 = vfrag(j), v1 = vfrag(j + 1);
-    if constexpr (PACK) {
-      const bool hi = c < 8;
-      const f16x8 pb = f16x8_of(make_uint4(hi ? ph[0][0] : plo[0][0], hi ? ph[0][1] : plo[0][1],
-                                           hi ? ph[0][2] : plo[0][2], hi ? ph[0][3] : plo[0][3]));
-      st.acc[0][j] = mfma16(v0, pb, st.acc[0][j]);
-      st.acc[0][j + 1] = mfma16(v1, pb, st.acc[0][j + 1]);
-    } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      st.acc[n][j] = mfma16(v0, ph[n], st.acc[n][j]);
+      st.acc[n][j + 1] = mfma16(v1, ph[n], st.acc[n][j + 1]);
+    }
+    if constexpr (!PACK) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const f16x8 pb = f16x8_of(make_uint4(ph[n][0], ph[n][1], ph[n][2], ph[n][3]));
-        st.acc[n][j] = mfma16(v0, pb, st.acc[n][j]);
-        st.acc[n][j + 1] = mfma16(v1, pb, st.acc[n][j + 1]);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const f16x8 pb = f16x8_of(make_uint4(plo[n][0], plo[n][1], plo[n][2], plo[n][3]));
-        st.acc[n][j] = mfma16(v0, pb, st.acc[n][j]);
-        st.acc[n][j + 1] = mfma16(v1, pb, st.acc[n][j + 1]);
+        st.acc[n][j] = mfma16(v0, pl[n], st.acc[n][j]);
+        st.acc[n][j + 1] = mfma16(v1, pl[n], st.acc[n][j + 1]);
       }
     }
   }
@@ -642,11 +653,12 @@ __device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride, int j) {
 // Otherwise a sequence's own keys; with one split (and the prefix's partial
 // results, where there are) the block writes the output itself.
 template <int ROW, bool PACK, int WAVES, bool SHARED>
-__global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan pl) {
+__global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ8Args a, AttnQ8Plan pl) {
   constexpr int KS = ROW / 32;       // MFMA steps of a score
   constexpr int DT = ROW / 16;       // MFMAs of 16 output columns
   constexpr int RT = PACK ? 8 : 16;  // rows of a job
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
   Job<SHARED> job;
   job.init(a, pl);
@@ -658,15 +670,31 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
   const int8_t* kep = src.ke + base;
   const int8_t* vep = src.ve + base;
 
-  // q, and with one split the first tile (inside the cache wherever the rows
-  // end), are under way before the lengths have arrived.
-  const RowRef ref = job.row(a, row0 + (PACK ? c & 7 : c));
-  RawQ<ROW> raw;
-  raw.load(a, ref, g);
-  Tile<ROW> cur;
+  // With one split the first tile (inside the cache wherever the rows end) is
+  // under way before the lengths have arrived.
+  Tile<ROW> even, odd;  // the wave's tiles in turn
   const bool early = job.splits == 1;
-  if (early)
-    load_tile<ROW>(cur, kp, vp, kep, vep, min((uint32_t)wave * 32, src.cap - 32), g, c);
+  if (early) {
+    const uint32_t key = min((uint32_t)wave * 32, src.cap - 32);
+    load_k<ROW>(even, kp, kep, vep, key, g, c);
+    load_v<ROW>(even, vp, key, g, c);
+  }
+  // Wave 0 makes the rows' operands for all.
+  __shared__ uint4 sq[PACK ? 1 : 2][KS][64];
+  __shared__ float sqf[16];
+  const RowRef ref = job.row(a, row0 + (PACK ? c & 7 : c));
+  if (wave == 0) {
+    RawQ<ROW> raw;
+    raw.load(a, ref, g);
+    f16x8 hi[KS], lo[KS];
+    const float f = raw.operands(a, hi, lo);
+    if (g == 0) sqf[c] = f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      sq[0][s][lane] = __builtin_bit_cast(uint4, PACK && c >= 8 ? lo[s] : hi[s]);
+      if constexpr (!PACK) sq[1][s][lane] = __builtin_bit_cast(uint4, lo[s]);
+    }
+  }
   // The split's tiles [t0, t1), the waves' in turn.
   uint32_t least, most;
   job.span(a, row0, RT, least, most);
@@ -674,19 +702,26 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
   const uint32_t per = early ? tiles : (tiles + job.splits - 1) / job.splits;
   const uint32_t t0 = min(tiles, job.split * per), t1 = min(tiles, t0 + per);
   uint32_t t = t0 + wave;
-  if (!early && t < t1) load_tile<ROW>(cur, kp, vp, kep, vep, t * 32, g, c);
-
-  f16x8 qh[1][KS], ql[1][KS];
-  const float qf = raw.operands(a, qh[0], ql[0]);
-  if constexpr (PACK) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qh[0][s] = c < 8 ? qh[0][s] : ql[0][s];
+  if (!early && t < t1) {
+    load_k<ROW>(even, kp, kep, vep, t * 32, g, c);
+    load_v<ROW>(even, vp, t * 32, g, c);
   }
+  if (t + WAVES < t1) {
+    load_k<ROW>(odd, kp, kep, vep, (t + WAVES) * 32, g, c);
+    load_v<ROW>(odd, vp, (t + WAVES) * 32, g, c);
+  }
+  __syncthreads();
+  f16x8 qh[1][KS], ql[1][KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    qh[0][s] = f16x8_of(sq[0][s][lane]);
+    if constexpr (!PACK) ql[0][s] = f16x8_of(sq[1][s][lane]);
+  }
+  const float qf = sqf[c];
   RowsState<ROW, 1> st;
   st.init();
-  for (; t < t1; t += WAVES) {
-    Tile<ROW> next;
-    load_tile<ROW>(next, kp, vp, kep, vep, min(t + WAVES, t1 - 1) * 32, g, c);
+  auto step = [&](Tile<ROW>& tile) {
+    uint32_t ke[2] = {tile.ke[0], tile.ke[1]}, ve[2] = {tile.ve[0], tile.ve[1]};
     if (t * 32 + 32 > most) {  // behind the rows' last key the exponents may be anything
       asm volatile("");
 #pragma unroll
@@ -694,32 +729,36 @@ __global__ __launch_bounds__(64 * WAVES) void k_attn_q8(AttnQ8Args a, AttnQ8Plan
         const uint32_t key = t * 32 + 16 * hh + 4 * g;
         const int left = (int)min(most, key + 4) - (int)key;
         const uint32_t keep = left <= 0 ? 0u : 0xFFFFFFFFu >> (32 - 8 * left);
-        cur.ke[hh] = (cur.ke[hh] & keep) | (0x82828282u & ~keep);
-        cur.ve[hh] = (cur.ve[hh] & keep) | (0x82828282u & ~keep);
+        ke[hh] &= keep;
+        ve[hh] &= keep;
       }
     }
-    const uint32_t bk[2] = {biased(cur.ke[0]), biased(cur.ke[1])};
-    const uint32_t bv[2] = {biased(cur.ve[0]), biased(cur.ve[1])};
-    uint32_t nan = 0;  // a byte of 255
+    const i32x4 e0 = exps_of(ke[0]), e1 = exps_of(ke[1]), f0 = exps_of(ve[0]), f1 = exps_of(ve[1]);
+    int low = 0, high = 0;
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
-      nan |= ((~bk[hh] - 0x01010101u) & bk[hh]) | ((~bv[hh] - 0x01010101u) & bv[hh]);
+    for (int r = 0; r < 4; ++r) {
+      low = min(low, min(min(e0[r], e1[r]), min(f0[r], f1[r])));
+      high = max(high, max(e0[r], e1[r]));
+    }
+    const bool more = t + 2 * WAVES < t1;
     tile_step<ROW, 1, PACK>(
-        st, qh, ql, &qf, &ref.limit, least, t, g, c, __any(nan & 0x80808080u),
+        st, qh, ql, &qf, &ref.limit, least, t, g, c, __any(low == kNanExp || high >= kBigExp),
         [&](int hh, int s) {
-          const uint4 w = cur.k[hh][s >> 1];
+          const uint4 w = tile.k[hh][s >> 1];
           return (s & 1) ? codes8_f16(w.z, w.w) : codes8_f16(w.x, w.y);
         },
-        [&](int j) { return v_frag(&cur.v[0][j / 4], ROW / 64, j); },
-        [&](int hh) {
-          return f32x4{biased_power(bk[hh], 0), biased_power(bk[hh], 1), biased_power(bk[hh], 2),
-                       biased_power(bk[hh], 3)};
-        },
-        [&](int hh) {
-          return f32x4{biased_power(bv[hh], 0), biased_power(bv[hh], 1), biased_power(bv[hh], 2),
-                       biased_power(bv[hh], 3)};
+        [&](int j) { return v_frag(&tile.v[0][j / 4], ROW / 64, j); },
+        [&](int hh) { return hh ? e1 : e0; }, [&](int hh) { return hh ? f1 : f0; },
+        [&]() {  // its registers take the wave's next tile but one
+          if (more) load_k<ROW>(tile, kp, kep, vep, (t + 2 * WAVES) * 32, g, c);
         });
-    cur = next;
+    if (more) load_v<ROW>(tile, vp, (t + 2 * WAVES) * 32, g, c);
+    t += WAVES;
+  };
+  while (t < t1) {
+    step(even);
+    if (t >= t1) break;
+    step(odd);
   }
 
   // Join the waves: each one's row normalised, weighted by its sum; and with
@@ -837,9 +876,10 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   constexpr size_t kBuffers = (size_t)2 * 2 * FRAGS * 64;  // in uint4
   constexpr size_t kJoin = (size_t)RW * 32 * RS / 4 + RW * 16;
   __shared__ uint4 smem[kBuffers > kJoin ? kBuffers : kJoin];
-  __shared__ __attribute__((aligned(16))) float scales[2][2][64];  // 2^e of a stage's keys, K's and V's
-  __shared__ uint32_t nans[2][2];         // the NaN rows of its tiles
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ __attribute__((aligned(16))) int exps[2][2][64];  // a stage's exponents, K's and V's
+  __shared__ uint32_t odds[2][2];  // whether its tiles are odd
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
   const int rw = wave % RW, kw = wave / RW;
   Job<SHARED> job;
@@ -898,8 +938,8 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     if (wave == W - 1) {
       const uint32_t key = min(t + lane / 32, t1 - 1) * 32 + lane % 32;
       const bool in = key < most;  // behind that there may be anything
-      re[0] = in ? kep[key] : -126;
-      re[1] = in ? vep[key] : -126;
+      re[0] = in ? kep[key] : 0;
+      re[1] = in ? vep[key] : 0;
     }
   };
   auto store = [&](int half) {
@@ -925,10 +965,10 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
       }
     }
     if (wave == W - 1) {
-      scales[half][0][lane] = __uint_as_float((uint32_t)(re[0] + 127) << 23 & 0x7F800000u);
-      scales[half][1][lane] = __uint_as_float((uint32_t)(re[1] + 127) << 23 & 0x7F800000u);
-      const uint64_t nan = __ballot(re[0] == kNanExp || re[1] == kNanExp);
-      if (lane < 2) nans[half][lane] = (uint32_t)(nan >> (32 * lane));
+      exps[half][0][lane] = re[0];
+      exps[half][1][lane] = re[1];
+      const uint64_t odd = __ballot(re[0] == kNanExp || re[1] == kNanExp || re[0] >= kBigExp);
+      if (lane < 2) odds[half][lane] = (uint32_t)(odd >> (32 * lane));
     }
   };
 
@@ -944,14 +984,14 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     if (t + 2 < t1) load(t + 2);
     if (t + kw < t1 && (t + kw) * 32 < mine) {
       const uint4* f = smem + ((size_t)half * 2 + kw) * FRAGS * 64 + lane;
-      const float* sk = &scales[half][0][32 * kw + 4 * g];
+      const int* e = &exps[half][0][32 * kw + 4 * g];
       tile_step<ROW, NT, false>(
           st, qh, ql, qf, limit, least, t + kw, g, c,
-          __builtin_amdgcn_readfirstlane(nans[half][kw]) != 0,
+          __builtin_amdgcn_readfirstlane(odds[half][kw]) != 0,
           [&](int hh, int s) { return f16x8_of(f[(hh * KS + s) * 64]); },
           [&](int j) { return f16x8_of(f[(2 * KS + j) * 64]); },
-          [&](int hh) { return *reinterpret_cast<const f32x4*>(sk + 16 * hh); },
-          [&](int hh) { return *reinterpret_cast<const f32x4*>(sk + 64 + 16 * hh); });
+          [&](int hh) { return *reinterpret_cast<const i32x4*>(e + 16 * hh); },
+          [&](int hh) { return *reinterpret_cast<const i32x4*>(e + 64 + 16 * hh); }, []() {});
     }
     half ^= 1;
     if (t + 2 < t1) store(half);
