@@ -459,19 +459,21 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   f32x4 d[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f16x8 k0 = kfrag(0, 0), k1 = kfrag(1, 0);
 #pragma unroll
   for (int s = 0; s < KS; ++s) {  // both halves' products in turn: no MFMA waits for the last one
-    const f16x8 k0 = kfrag(0, s), k1 = kfrag(1, s);
+    f16x8 m0 = k0, m1 = k1;
+    if (s + 1 < KS) k0 = kfrag(0, s + 1), k1 = kfrag(1, s + 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      d[n][0] = mfma16(k0, qh[n][s], d[n][0]);
-      d[n][1] = mfma16(k1, qh[n][s], d[n][1]);
+      d[n][0] = mfma16(m0, qh[n][s], d[n][0]);
+      d[n][1] = mfma16(m1, qh[n][s], d[n][1]);
     }
     if constexpr (!PACK) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        d[n][0] = mfma16(k0, ql[n][s], d[n][0]);
-        d[n][1] = mfma16(k1, ql[n][s], d[n][1]);
+        d[n][0] = mfma16(m0, ql[n][s], d[n][0]);
+        d[n][1] = mfma16(m1, ql[n][s], d[n][1]);
       }
     }
   }
@@ -490,7 +492,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   float qe[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) qe[n] = qf[n];
-  int plain = 1;  // 0: K's exponents are applied already
+  int plain = -1;  // 0: K's exponents are applied already
   if (odd) {
     asm volatile("");
 #pragma unroll
@@ -510,7 +512,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     for (int n = 0; n < NT; ++n) add[n] = 0.f;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
-      const i32x4 ke = kexp(hh) * plain;
+      const i32x4 ke = kexp(hh) & plain;
       i32x4 ve = vexp(hh);
       if (st.eb != 0) {
         asm volatile("");
@@ -560,7 +562,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x = ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] * plain) * qe[n];
+        const float x = ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] & plain) * qe[n];
         const bool in = sees(n, i);
         mx = fmaxf(mx, in ? x : -INFINITY);
         mw = fmaxf(mw, in ? x + (float)vexp(i >> 2)[i & 3] : -INFINITY);
@@ -615,19 +617,21 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     ph[n] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
   }
   // O^T += V^T P^T.
+  f16x8 v0 = vfrag(0), v1 = vfrag(1);
 #pragma unroll
   for (int j = 0; j < DT; j += 2) {
-    const f16x8 v0 = vfrag(j), v1 = vfrag(j + 1);
+    const f16x8 m0 = v0, m1 = v1;
+    if (j + 2 < DT) v0 = vfrag(j + 2), v1 = vfrag(j + 3);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      st.acc[n][j] = mfma16(v0, ph[n], st.acc[n][j]);
-      st.acc[n][j + 1] = mfma16(v1, ph[n], st.acc[n][j + 1]);
+      st.acc[n][j] = mfma16(m0, ph[n], st.acc[n][j]);
+      st.acc[n][j + 1] = mfma16(m1, ph[n], st.acc[n][j + 1]);
     }
     if constexpr (!PACK) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        st.acc[n][j] = mfma16(v0, pl[n], st.acc[n][j]);
-        st.acc[n][j + 1] = mfma16(v1, pl[n], st.acc[n][j + 1]);
+        st.acc[n][j] = mfma16(m0, pl[n], st.acc[n][j]);
+        st.acc[n][j + 1] = mfma16(m1, pl[n], st.acc[n][j + 1]);
       }
     }
   }
@@ -886,18 +890,6 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   job.init(a, pl);
   const Q8Cache& src = SHARED ? a.pre : a.c;
   const uint32_t row0 = job.group * 32 * RW + rw * 32;
-  RowRef ref[NT];
-  uint32_t limit[NT];
-  f16x8 qh[NT][KS], ql[NT][KS];
-  float qf[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    ref[n] = job.row(a, row0 + n * 16 + c);
-    limit[n] = ref[n].limit;
-    RawQ<ROW> raw;
-    raw.load(a, ref[n], g);
-    qf[n] = raw.operands(a, qh[n], ql[n]);
-  }
   // The wave's rows, and as far as the block's furthest one.
   uint32_t least, mine, unused, most;
   job.span(a, row0, 32, least, mine);
@@ -972,12 +964,22 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     }
   };
 
+  if (t0 < t1) load(t0);
+  RowRef ref[NT];
+  uint32_t limit[NT];
+  f16x8 qh[NT][KS], ql[NT][KS];
+  float qf[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    ref[n] = job.row(a, row0 + n * 16 + c);
+    limit[n] = ref[n].limit;
+    RawQ<ROW> raw;
+    raw.load(a, ref[n], g);
+    qf[n] = raw.operands(a, qh[n], ql[n]);
+  }
   RowsState<ROW, NT> st;
   st.init();
-  if (t0 < t1) {
-    load(t0);
-    store(0);
-  }
+  if (t0 < t1) store(0);
   int half = 0;
   for (uint32_t t = t0; t < t1; t += 2) {
     __syncthreads();
