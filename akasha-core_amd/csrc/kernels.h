@@ -581,8 +581,9 @@ struct AttnQ8Args {
 constexpr uint32_t kAttnMaxSplits = 64;
 struct AttnQ8Plan {
   uint32_t G;                                        // query heads of a kv head
-  uint32_t own_rt, own_groups, own_splits;           // rows a job, jobs, splits of the keys
-  uint32_t prefix_rt, prefix_groups, prefix_splits;  // splits 0: no prefix
+  // Rows of a job, jobs for all rows, splits of the keys, waves of a block.
+  uint32_t own_rt, own_groups, own_splits, own_waves;
+  uint32_t prefix_rt, prefix_groups, prefix_splits, prefix_waves;  // splits 0: no prefix
   size_t rows_offset, bytes;  // the workspace: maxima and sums, then rows
 };
 size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix);

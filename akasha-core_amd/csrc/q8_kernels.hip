@@ -362,54 +362,50 @@ struct RawQ {
         for (int i = 0; i < 8; i += 4) {
           const int d = (s >> 1) * 64 + 16 * g + 8 * (s & 1) + i;
           const float4 u = *reinterpret_cast<const float4*>(q + min(d, hd - 4));
-          const bool in = d < hd;
-          x[s][i] = in ? u.x : 0.f;
-          x[s][i + 1] = in ? u.y : 0.f;
-          x[s][i + 2] = in ? u.z : 0.f;
-          x[s][i + 3] = in ? u.w : 0.f;
+          x[s][i] = u.x;
+          x[s][i + 1] = u.y;
+          x[s][i + 2] = u.z;
+          x[s][i + 3] = u.w;
         }
     } else {
 #pragma unroll
       for (int s = 0; s < ROW / 32; ++s)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = (s >> 1) * 64 + 16 * g + 8 * (s & 1) + i;
-          const float u = q[min(d, hd - 1)];
-          x[s][i] = d < hd ? u : 0.f;
-        }
+        for (int i = 0; i < 8; ++i)
+          x[s][i] = q[min((s >> 1) * 64 + 16 * g + 8 * (s & 1) + i, hd - 1)];
+    }
+    if (hd != ROW) {
+#pragma unroll
+      for (int s = 0; s < ROW / 32; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((s >> 1) * 64 + 16 * g + 8 * (s & 1) + i >= hd) x[s][i] = 0.f;
     }
   }
 
-  // As B operands, hi and lo, scaled by scale log2(e) and by 2^-e to a largest
-  // magnitude in [2^13, 2^14); returns 2^e, NaN for a row with a NaN or an
-  // infinity.
+  // As B operands, hi and lo, times scale log2(e) 2^-e with a largest magnitude
+  // in [2^13, 2^14] or next to it; returns 2^e.  A NaN or an infinity makes one
+  // of the terms NaN (inf - inf), and with it the row's scores.
   __device__ __forceinline__ float operands(const AttnQ8Args& a, f16x8* hi, f16x8* lo) {
-    float top = 0.f, sum = 0.f;
+    float top = 0.f;
 #pragma unroll
     for (int s = 0; s < ROW / 32; ++s)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[s][i] *= a.scale_log2;
-        top = fmaxf(top, fabsf(x[s][i]));
-        sum += x[s][i] * 0.f;  // NaN where anything is not finite
-      }
-    top = xor_max<32>(xor_max<16>(top));
-    sum = xor_sum<32>(xor_sum<16>(sum));
-    // top = 1.m 2^(E - 127); times 2^(140 - E) it is 1.m 2^13 (E at least 15, so
-    // that both powers are normal numbers; smaller rows keep small terms).
-    const int E = max(15, (int)(__float_as_uint(top) >> 23));
-    const float s1 = ldexpf(1.f, 140 - E), back = ldexpf(1.f, E - 140);
-    const bool ok = sum == 0.f;
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[s][i]));
+    top = xor_max<32>(xor_max<16>(top)) * fabsf(a.scale_log2);
+    // top = 1.m 2^(E - 127); times 2^(140 - E) it is 1.m 2^13 (E at least 40, so
+    // that the factor is a normal number; smaller rows keep small terms).
+    const int E = max(40, (int)(__float_as_uint(top) >> 23));
+    const float f = ldexpf(a.scale_log2, 140 - E);
 #pragma unroll
     for (int s = 0; s < ROW / 32; ++s) {
       uint32_t h[4], l[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        split2(ok ? x[s][2 * i] * s1 : 0.f, ok ? x[s][2 * i + 1] * s1 : 0.f, h[i], l[i]);
+      for (int i = 0; i < 4; ++i) split2(x[s][2 * i] * f, x[s][2 * i + 1] * f, h[i], l[i]);
       hi[s] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
       lo[s] = f16x8_of(make_uint4(l[0], l[1], l[2], l[3]));
     }
-    return ok ? back : __int_as_float(0x7FC00000);
+    return ldexpf(1.f, E - 140);
   }
 };
 
@@ -653,6 +649,20 @@ __device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride, int j) {
   }
 }
 
+// Four columns of a row's output, as many as the head has.
+__device__ __forceinline__ void store_out(const AttnQ8Args& a, const RowRef& x, uint32_t col,
+                                          f32x4 v) {
+  const uint32_t hd = a.c.head_dim;
+  float* out = a.out + x.bt * a.out_stride + (size_t)x.head * hd + col;
+  if (a.out_vec) {
+    if (col < hd) *reinterpret_cast<f32x4*>(out) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < hd) out[i] = v[i];
+  }
+}
+
 // SHARED: the prefix's keys for the rows of all sequences, as partial results.
 // Otherwise a sequence's own keys; with one split (and the prefix's partial
 // results, where there are) the block writes the output itself.
@@ -682,6 +692,26 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     const uint32_t key = min((uint32_t)wave * 32, src.cap - 32);
     load_k<ROW>(even, kp, kep, vep, key, g, c);
     load_v<ROW>(even, vp, key, g, c);
+  }
+  // The prefix's parts of the job's rows, 64 WAVES / RT lanes to a row.
+  constexpr int L = 64 * WAVES / RT;
+  constexpr int MAXP = SHARED ? 0 : kAttnMaxSplits, NP = (MAXP + L - 1) / L;
+  const bool final = !SHARED && pl.own_splits == 1;
+  const uint32_t extra = final ? pl.prefix_splits : 0;
+  PartMl* ml = reinterpret_cast<PartMl*>(a.ws);
+  float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
+  const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
+  const int jrow = threadIdx.x / L, jl = threadIdx.x % L;
+  PartMl pre[NP > 0 ? NP : 1];
+  if (NP > 0 && extra) {
+    const RowRef x = job.row(a, row0 + jrow);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      pre[i] = x.live && jl + i * L < (int)extra ? ml[row_id(a, x) * nparts + jl + i * L]
+                                                 : PartMl{-INFINITY, 0.f};
+  } else {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) pre[i] = {-INFINITY, 0.f};
   }
   // Wave 0 makes the rows' operands for all.
   __shared__ uint4 sq[PACK ? 1 : 2][KS][64];
@@ -765,26 +795,13 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     step(odd);
   }
 
-  // Join the waves: each one's row normalised, weighted by its sum; and with
-  // them the prefix's parts, 64 WAVES / RT lanes to a row.
-  constexpr int RS = ROW + 4, L = 64 * WAVES / RT;
-  constexpr int MAXP = SHARED ? 0 : kAttnMaxSplits, NP = (MAXP + L - 1) / L;
-  __shared__ float so[WAVES][RT][RS];
+  // Join the waves and the prefix's parts: rows normalised, weighted by sums.
+  constexpr int RS = ROW + 4;
+  constexpr int EL = (RT * (ROW / 4) + 64 * WAVES - 1) / (64 * WAVES);  // quads of columns a thread
+  __shared__ __attribute__((aligned(16))) float so[WAVES][RT][RS];
   __shared__ PartMl sml[WAVES][RT];
   __shared__ float sw[RT][WAVES + MAXP];
   __shared__ float2 sfin[RT];  // maximum and sum of a row over all its parts
-  const bool final = !SHARED && pl.own_splits == 1;
-  const uint32_t extra = final ? pl.prefix_splits : 0;
-  PartMl* ml = reinterpret_cast<PartMl*>(a.ws);
-  float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
-  const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
-  const int jrow = threadIdx.x / L, jl = threadIdx.x % L;
-  const RowRef jref = job.row(a, row0 + jrow);
-  PartMl pre[NP > 0 ? NP : 1];
-#pragma unroll
-  for (int i = 0; i < NP; ++i)
-    pre[i] = jref.live && jl + i * L < (int)extra ? ml[row_id(a, jref) * nparts + jl + i * L]
-                                                  : PartMl{-INFINITY, 0.f};
   const float total = xor_sum<32>(xor_sum<16>(st.l[0]));
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const bool mine = !PACK || c < 8;
@@ -793,17 +810,38 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int j = 0; j < DT; j += 4) {
-      float o[4];
+      f32x4 o;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[i] = st.acc[0][j + i][r];
         if constexpr (PACK) o[i] += dpp_f32<0x128>(o[i]);
-        o[i] = ldexpf(o[i] * inv, st.eb);
+        o[i] *= inv;
       }
-      if (mine && ref.live)
-        *reinterpret_cast<float4*>(&so[wave][c][(4 * g + r) * DT + j]) =
-            make_float4(o[0], o[1], o[2], o[3]);
+      if (st.eb != 0) {
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], st.eb);
+      }
+      if (mine && ref.live) *reinterpret_cast<f32x4*>(&so[wave][c][(4 * g + r) * DT + j]) = o;
     }
+  // The thread's quads of columns, and the parts' of the first eight splits.
+  const uint32_t hd = a.c.head_dim;
+  const uint32_t rows_here = min((uint32_t)RT, job.nrows - row0);
+  RowRef xr[EL];
+  const float* pq[EL];
+  f32x4 pv[EL][8];
+#pragma unroll
+  for (int e = 0; e < EL; ++e) {
+    const uint32_t id = threadIdx.x + e * 64 * WAVES;
+    xr[e] = job.row(a, row0 + id / (ROW / 4));
+    xr[e].live = xr[e].live && id / (ROW / 4) < rows_here;
+    pq[e] = po + row_id(a, xr[e]) * nparts * ROW + id % (ROW / 4) * 4;
+    if constexpr (!SHARED) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p)
+        if (p < (int)extra && xr[e].live) pv[e][p] = *reinterpret_cast<const f32x4*>(pq[e] + p * ROW);
+    }
+  }
   __syncthreads();
   {
     const PartMl y = jl < WAVES ? sml[jl][jrow] : PartMl{-INFINITY, 0.f};
@@ -812,8 +850,7 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     for (int i = 0; i < NP; ++i) m = fmaxf(m, pre[i].m);
     m = group_max<L>(m);
     const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
-    float sum = f;
-    float z[NP > 0 ? NP : 1];
+    float sum = f, z[NP > 0 ? NP : 1];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       z[i] = pre[i].l == 0.f ? 0.f : pre[i].l * __builtin_amdgcn_exp2f(pre[i].m - m);
@@ -828,37 +865,35 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     if (jl == 0) sfin[jrow] = make_float2(m, sum);
   }
   __syncthreads();
-  const uint32_t hd = a.c.head_dim;
-  const uint32_t rows_here = min((uint32_t)RT, job.nrows - row0);
   const uint32_t at = SHARED ? job.split : pl.prefix_splits + job.split;
-  for (uint32_t e = threadIdx.x; e < rows_here * ROW; e += 64 * WAVES) {
-    const uint32_t row = e / ROW, col = e % ROW;
-    if (col >= hd) continue;
-    const RowRef x = job.row(a, row0 + row);
-    const float2 fin = sfin[row];
-    float o = 0.f;
-    if (x.live && fin.y != 0.f) {
-      if constexpr (!SHARED) {
-        const float* q = po + row_id(a, x) * nparts * ROW + col;
-#pragma unroll 8
-        for (uint32_t p = 0; p < extra; ++p) {
-          const float f = sw[row][WAVES + p], y = q[(size_t)p * ROW];
-          o += f == 0.f ? 0.f : f * y;  // an empty part's row may hold anything
-        }
-      }
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        const float f = sw[row][w];
-        o += f == 0.f ? 0.f : f * so[w][row][col];
+  for (int e = 0; e < EL; ++e) {
+    const uint32_t id = threadIdx.x + e * 64 * WAVES;
+    const uint32_t row = id / (ROW / 4), col = id % (ROW / 4) * 4;
+    if (row >= rows_here) continue;
+    const RowRef x = xr[e];
+    const float2 fin = sfin[row];
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (x.live) {  // (parts without a key are zeros)
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+        o += sw[row][w] * *reinterpret_cast<const f32x4*>(&so[w][row][col]);
+      if constexpr (!SHARED) {
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+          if (p < (int)extra) o += sw[row][WAVES + p] * pv[e][p];
+#pragma unroll 4
+        for (uint32_t p = 8; p < extra; ++p)
+          o += sw[row][WAVES + p] * *reinterpret_cast<const f32x4*>(pq[e] + (size_t)p * ROW);
       }
     }
     if (final) {
-      a.out[x.bt * a.out_stride + (size_t)x.head * hd + col] = x.live ? o : 0.f;
+      store_out(a, x, col, o);
       if (col == 0 && a.lse)
         a.lse[row_id(a, x)] =
             x.live && fin.y != 0.f ? (fin.x + log2f(fin.y)) * 0.6931471805599453f : -INFINITY;
     } else if (x.live) {
-      po[(row_id(a, x) * nparts + at) * ROW + col] = o;
+      *reinterpret_cast<f32x4*>(po + (row_id(a, x) * nparts + at) * ROW + col) = o;
       if (col == 0) ml[row_id(a, x) * nparts + at] = {fin.y == 0.f ? -INFINITY : fin.x, fin.y};
     }
   }
@@ -882,6 +917,8 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   __shared__ uint4 smem[kBuffers > kJoin ? kBuffers : kJoin];
   __shared__ __attribute__((aligned(16))) int exps[2][2][64];  // a stage's exponents, K's and V's
   __shared__ uint32_t odds[2][2];  // whether its tiles are odd
+  __shared__ float sqf[32 * RW];
+  static_assert((size_t)W * KS * 2 * 64 <= kBuffers, "the rows' operands fit the buffers");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
@@ -965,18 +1002,37 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   };
 
   if (t0 < t1) load(t0);
+  // The rows' operands, 16 rows a wave, by way of the buffer.
+  {
+    const RowRef x = job.row(a, job.group * 32 * RW + wave * 16 + c);
+    RawQ<ROW> raw;
+    raw.load(a, x, g);
+    f16x8 hi[KS], lo[KS];
+    const float f = raw.operands(a, hi, lo);
+    if (g == 0) sqf[wave * 16 + c] = f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      smem[((wave * KS + s) * 2) * 64 + lane] = __builtin_bit_cast(uint4, hi[s]);
+      smem[((wave * KS + s) * 2 + 1) * 64 + lane] = __builtin_bit_cast(uint4, lo[s]);
+    }
+  }
   RowRef ref[NT];
   uint32_t limit[NT];
   f16x8 qh[NT][KS], ql[NT][KS];
   float qf[NT];
+  __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     ref[n] = job.row(a, row0 + n * 16 + c);
     limit[n] = ref[n].limit;
-    RawQ<ROW> raw;
-    raw.load(a, ref[n], g);
-    qf[n] = raw.operands(a, qh[n], ql[n]);
+    qf[n] = sqf[rw * 32 + n * 16 + c];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qh[n][s] = f16x8_of(smem[(((rw * 2 + n) * KS + s) * 2) * 64 + lane]);
+      ql[n][s] = f16x8_of(smem[(((rw * 2 + n) * KS + s) * 2 + 1) * 64 + lane]);
+    }
   }
+  __syncthreads();
   RowsState<ROW, NT> st;
   st.init();
   if (t0 < t1) store(0);
@@ -999,7 +1055,8 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     if (t + 2 < t1) store(half);
   }
 
-  // The second tiles' waves hand their normalised rows to the first's.
+  // The two waves of the same rows exchange 16 rows each, normalised, and
+  // finish the other 16.
   __syncthreads();
   float* so = reinterpret_cast<float*>(smem);
   PartMl* sml = reinterpret_cast<PartMl*>(so + (size_t)RW * 32 * RS);
@@ -1010,105 +1067,85 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     m[n] = total[n] == 0.f ? -INFINITY : st.mt[n];
     const float inv = total[n] == 0.f ? 0.f : 1.f / total[n];
 #pragma unroll
-    for (int j = 0; j < DT; ++j)
+    for (int j = 0; j < DT; ++j) st.acc[n][j] *= inv;
+    if (st.eb != 0) {
+      asm volatile("");
 #pragma unroll
-      for (int r = 0; r < 4; ++r) st.acc[n][j][r] = ldexpf(st.acc[n][j][r] * inv, st.eb);
-    const int row = rw * 32 + n * 16 + c;
-    if (kw == 1) {
-      if (g == 0) sml[row] = {m[n], total[n]};
+      for (int j = 0; j < DT; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < DT; j += 4)
-          *reinterpret_cast<float4*>(so + (size_t)row * RS + (4 * g + r) * DT + j) =
-              make_float4(st.acc[n][j][r], st.acc[n][j + 1][r], st.acc[n][j + 2][r],
-                          st.acc[n][j + 3][r]);
+        for (int r = 0; r < 4; ++r) st.acc[n][j][r] = ldexpf(st.acc[n][j][r], st.eb);
     }
   }
+  const int row = rw * 32 + c;  // + 16 for the rows of kw = 1
+  auto hand = [&](const f32x4* acc, float mm, float ll, int r16) {
+    if (g == 0) sml[row + r16] = {mm, ll};
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < DT; j += 4)
+        *reinterpret_cast<f32x4*>(so + (size_t)(row + r16) * RS + (4 * g + r) * DT + j) =
+            f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+  };
+  if (kw == 0)
+    hand(st.acc[1], m[1], total[1], 16);
+  else
+    hand(st.acc[0], m[0], total[0], 0);
   __syncthreads();
-  if (kw == 1) return;
   const bool final = !SHARED && pl.own_splits == 1;
   const uint32_t extra = final ? pl.prefix_splits : 0;
   PartMl* ml = reinterpret_cast<PartMl*>(a.ws);
   float* po = reinterpret_cast<float*>(static_cast<char*>(a.ws) + pl.rows_offset);
   const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
   const uint32_t at = SHARED ? job.split : pl.prefix_splits + job.split;
-  const uint32_t hd = a.c.head_dim;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const RowRef x = ref[n];
-    if (row0 + n * 16 + c >= job.nrows || (!x.live && !final)) continue;
-    const int row = rw * 32 + n * 16 + c;
+  auto finish = [&](f32x4* acc, float mm, float ll, const RowRef& x, int r16) {
+    if (row0 + r16 + c >= job.nrows || (!x.live && !final)) return;
     const size_t part = row_id(a, x) * nparts;
-    const PartMl y = sml[row];
-    float top = fmaxf(m[n], y.m);
+    const PartMl y = sml[row + r16];
+    float top = fmaxf(mm, y.m);
     for (uint32_t e = 0; e < extra && x.live; ++e) top = fmaxf(top, ml[part + e].m);
-    const float f0 = total[n] == 0.f ? 0.f : total[n] * __builtin_amdgcn_exp2f(m[n] - top);
-    const float f1 = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - top);
     auto weight_of = [&](const PartMl& z) {
       return z.l == 0.f ? 0.f : z.l * __builtin_amdgcn_exp2f(z.m - top);
     };
+    const float f0 = weight_of({mm, ll}), f1 = weight_of(y);
     float sum = f0 + f1;
     for (uint32_t e = 0; e < extra && x.live; ++e) sum += weight_of(ml[part + e]);
-    const bool some = x.live && sum != 0.f;
-    const float inv = some ? 1.f / sum : 0.f;
-    const float n0 = f0 * inv, n1 = f1 * inv;
+    const float inv = x.live && sum != 0.f ? 1.f / sum : 0.f;
+    f32x4 o[DT];  // [r][j / 4]: columns (4 g + r) DT + j ..
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int j = 0; j < DT; j += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(so + (size_t)row * RS + (4 * g + r) * DT + j);
-        const float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float o = n0 == 0.f ? 0.f : n0 * st.acc[n][j + i][r];
-          if (n1 != 0.f) o += n1 * w[i];
-          st.acc[n][j + i][r] = o;
-        }
-      }
+      for (int j = 0; j < DT; j += 4)
+        o[r * (DT / 4) + j / 4] =
+            f0 * inv * f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]} +
+            f1 * inv *
+                *reinterpret_cast<const f32x4*>(so + (size_t)(row + r16) * RS + (4 * g + r) * DT + j);
     for (uint32_t e = 0; e < extra && x.live; ++e) {
       const float f = weight_of(ml[part + e]) * inv;
-      if (f == 0.f) continue;  // an empty part's row may hold anything
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < DT; j += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(po + (part + e) * ROW + (4 * g + r) * DT + j);
-          st.acc[n][j][r] += f * v.x;
-          st.acc[n][j + 1][r] += f * v.y;
-          st.acc[n][j + 2][r] += f * v.z;
-          st.acc[n][j + 3][r] += f * v.w;
-        }
+      for (int k = 0; k < DT; ++k)
+        o[k] += f * *reinterpret_cast<const f32x4*>(po + (part + e) * ROW + (4 * g) * DT + 4 * k);
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int j = 0; j < DT; j += 4) {
-        const float4 v = some ? make_float4(st.acc[n][j][r], st.acc[n][j + 1][r],
-                                            st.acc[n][j + 2][r], st.acc[n][j + 3][r])
-                              : make_float4(0.f, 0.f, 0.f, 0.f);
-        const uint32_t col = (4 * g + r) * DT + j;
-        if (!final) {
-          *reinterpret_cast<float4*>(po + (part + at) * ROW + col) = v;
-        } else {
-          float* out = a.out + x.bt * a.out_stride + (size_t)x.head * hd + col;
-          if (a.out_vec) {
-            if (col < hd) *reinterpret_cast<float4*>(out) = v;
-          } else {
-            if (col < hd) out[0] = v.x;
-            if (col + 1 < hd) out[1] = v.y;
-            if (col + 2 < hd) out[2] = v.z;
-            if (col + 3 < hd) out[3] = v.w;
-          }
-        }
-      }
+    for (int k = 0; k < DT; ++k) {
+      const uint32_t col = (4 * g) * DT + 4 * k;
+      if (!x.live) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!final)
+        *reinterpret_cast<f32x4*>(po + (part + at) * ROW + col) = o[k];
+      else
+        store_out(a, x, col, o[k]);
+    }
     if (g == 0) {
+      const bool some = x.live && sum != 0.f;
       if (!final)
         ml[part + at] = {some ? top : -INFINITY, some ? sum : 0.f};
       else if (a.lse)
         a.lse[row_id(a, x)] = some ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
-  }
+  };
+  if (kw == 0)
+    finish(st.acc[0], m[0], total[0], ref[0], 0);
+  else
+    finish(st.acc[1], m[1], total[1], ref[1], 16);
 }
 
 // Joins a row's partial results: one block per row and head, a wave takes
@@ -1148,7 +1185,7 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan p
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const float x = po[(size_t)p * ROW + 64 * i];
-        o[i] += w == 0.f ? 0.f : w * x;  // an empty part's row may hold anything
+        o[i] += w * x;  // (a part without a key is zeros)
       }
     }
   }
@@ -1203,12 +1240,40 @@ uint32_t rows_per_job(uint64_t rows) {
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
 }
 
-// Splits of `tiles` 32-key tiles among blocks, for `jobs` jobs of rt rows.
-uint32_t key_splits(uint64_t jobs, uint64_t tiles, uint32_t rt) {
-  const uint64_t want = rt <= 16 ? 1024 : rt <= 64 ? 512 : 256;
-  const uint64_t least = rt <= 16 ? 16 : 4;  // tiles that are worth a block
-  return (uint32_t)std::max<uint64_t>(
-      1, std::min<uint64_t>({kAttnMaxSplits, tiles / least, div_up(want, jobs)}));
+constexpr uint64_t kCus = 256;
+
+// Blocks' waves and the splits of `tiles` 32-key tiles for `jobs` jobs of rt
+// rows, from a model of the time in us.  Direct jobs: a block takes 4 us and
+// each of a wave's tiles 0.85 us alone, 2.75 with the CUs full (8 waves of 128
+// columns, 12 of 64, per CU); jobs in LDS: 8 us and 2.1 us a stage of two
+// tiles.  Several splits cost a join, and their rows written and read.
+struct Deal {
+  uint32_t waves, splits;
+};
+Deal deal(uint64_t jobs, uint64_t tiles, uint32_t rt, uint32_t row, uint64_t ids, bool joined) {
+  static const uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  Deal best{rt == 32 ? 2u : rt <= 64 ? 4u : 8u, 1};
+  double least = 1e30;
+  for (uint32_t w = rt <= 16 ? 2 : best.waves; w <= (rt <= 16 ? 4 : best.waves); w += 2)
+    for (uint32_t s : kSplits) {
+      if (s > kAttnMaxSplits || (s > 1 && tiles / s < (rt <= 16 ? 2 * w : 4))) break;
+      const double cap = (double)kCus * (rt > 16 ? (rt == 32 && row == 128 ? 4 : 8)
+                                                 : row == 64 ? 12 : 8);
+      const double full = (double)(jobs * s * w) / cap;
+      const double rounds = full <= 1 ? 1 : full <= 4 ? (double)(uint64_t)(full + 0.999) : full;
+      const double at_once = full < 1 ? full : 1;
+      const double per = (double)div_up(tiles, (uint64_t)s * w);
+      double t = rt <= 16 ? rounds * (4 + per * (0.85 + 1.9 * at_once))
+                          : rounds * (8 + (double)div_up(tiles, 2 * (uint64_t)s) * 2.1);
+      if (s > 1 || joined) t += (double)ids * s * row * 8 / 4e6;
+      if (s > 1 && !joined) t += 4;
+      if (t < least) {
+        least = t;
+        best.splits = s;
+        best.waves = w;
+      }
+    }
+  return best;
 }
 
 AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
@@ -1216,18 +1281,22 @@ AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   const uint64_t G = a.heads / a.c.kv_heads;
   p.G = (uint32_t)G;
   const uint64_t own = a.rows * G, all = own * a.batch;
+  const uint64_t ids = (uint64_t)a.batch * a.rows * a.heads;
   p.own_rt = rows_per_job(own);
   p.own_groups = (uint32_t)div_up(own, p.own_rt);
-  p.own_splits = key_splits((uint64_t)a.batch * a.c.kv_heads * p.own_groups,
-                            div_up(a.max_len, 32), p.own_rt);
-  if (prefix) {
+  const Deal d = deal((uint64_t)a.batch * a.c.kv_heads * p.own_groups, div_up(a.max_len, 32),
+                      p.own_rt, a.c.row, ids, false);
+  p.own_splits = d.splits;
+  p.own_waves = d.waves;
+  if (prefix) {  // its parts are joined with the own rows' in any case
     p.prefix_rt = rows_per_job(all);
     p.prefix_groups = (uint32_t)div_up(all, p.prefix_rt);
-    p.prefix_splits = key_splits((uint64_t)a.c.kv_heads * p.prefix_groups,
-                                 div_up(a.pre.max_rows, 32), p.prefix_rt);
+    const Deal e = deal((uint64_t)a.c.kv_heads * p.prefix_groups, div_up(a.pre.max_rows, 32),
+                        p.prefix_rt, a.c.row, ids, true);
+    p.prefix_splits = e.splits;
+    p.prefix_waves = e.waves;
   }
   const uint64_t parts = p.prefix_splits + (p.own_splits > 1 ? p.own_splits : 0);
-  const uint64_t ids = (uint64_t)a.batch * a.rows * a.heads;
   p.rows_offset = div_up(ids * parts * sizeof(PartMl), 16) * 16;
   p.bytes = parts ? p.rows_offset + ids * parts * a.c.row * sizeof(float) : 0;
   return p;
@@ -1238,12 +1307,13 @@ void launch_parts(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
   const uint32_t rt = SHARED ? p.prefix_rt : p.own_rt;
   const dim3 grid(SHARED ? p.prefix_groups * a.c.kv_heads * p.prefix_splits
                          : a.batch * p.own_splits * a.c.kv_heads * p.own_groups);
-  auto* f = rt == 8    ? k_attn_q8<ROW, true, 4, SHARED>
-            : rt == 16 ? k_attn_q8<ROW, false, 4, SHARED>
+  const uint32_t waves = SHARED ? p.prefix_waves : p.own_waves;
+  auto* f = rt == 8    ? (waves == 2 ? k_attn_q8<ROW, true, 2, SHARED> : k_attn_q8<ROW, true, 4, SHARED>)
+            : rt == 16 ? (waves == 2 ? k_attn_q8<ROW, false, 2, SHARED> : k_attn_q8<ROW, false, 4, SHARED>)
             : rt == 32 ? k_attn_q8_rows<ROW, 1, SHARED>
             : rt == 64 ? k_attn_q8_rows<ROW, 2, SHARED>
                        : k_attn_q8_rows<ROW, 4, SHARED>;
-  const uint32_t threads = rt <= 16 ? 256 : rt * 4;
+  const uint32_t threads = waves * 64;
   hipLaunchKernelGGL(f, grid, dim3(threads), 0, s, a, p);
 }
 
