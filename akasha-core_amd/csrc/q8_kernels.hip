@@ -383,6 +383,19 @@ struct RawQ {
     }
   }
 
+  // The same from 16 rows in LDS, `rs` floats apart.
+  __device__ __forceinline__ void from_lds(const float* rows, int rs, int g, int c) {
+#pragma unroll
+    for (int s = 0; s < ROW / 32; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(
+            rows + c * rs + (s >> 1) * 64 + 16 * g + 8 * (s & 1) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[s][i + k] = u[k];
+      }
+  }
+
   // As B operands, hi and lo, times scale log2(e) 2^-e with a largest magnitude
   // in [2^13, 2^14] or next to it; returns 2^e.  A NaN or an infinity makes one
   // of the terms NaN (inf - inf), and with it the row's scores.
@@ -649,11 +662,19 @@ __device__ __forceinline__ f16x8 v_frag(const uint32_t* v, int stride, int j) {
   }
 }
 
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t x, int lane) {
+  return (uint64_t)(uint32_t)__shfl((int)(x >> 32), lane, 64) << 32 |
+         (uint32_t)__shfl((int)(uint32_t)x, lane, 64);
+}
+
 // Four columns of a row's output, as many as the head has.
-__device__ __forceinline__ void store_out(const AttnQ8Args& a, const RowRef& x, uint32_t col,
+__device__ __forceinline__ uint64_t out_at(const AttnQ8Args& a, const RowRef& x) {
+  return x.bt * a.out_stride + (size_t)x.head * a.c.head_dim;
+}
+__device__ __forceinline__ void store_out(const AttnQ8Args& a, uint64_t at, uint32_t col,
                                           f32x4 v) {
   const uint32_t hd = a.c.head_dim;
-  float* out = a.out + x.bt * a.out_stride + (size_t)x.head * hd + col;
+  float* out = a.out + at + col;
   if (a.out_vec) {
     if (col < hd) *reinterpret_cast<f32x4*>(out) = v;
   } else {
@@ -888,7 +909,7 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
       }
     }
     if (final) {
-      store_out(a, x, col, o);
+      store_out(a, out_at(a, x), col, o);
       if (col == 0 && a.lse)
         a.lse[row_id(a, x)] =
             x.live && fin.y != 0.f ? (fin.x + log2f(fin.y)) * 0.6931471805599453f : -INFINITY;
@@ -944,6 +965,7 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   uint4 rk[KU];
   uint32_t rv[VU][8];
   int re[2] = {0, 0};  // exponents of key `lane` of the stage, the last wave's
+  bool re_in = false;
   auto load = [&](uint32_t t) {  // the stage of tiles t and t + 1
 #pragma unroll
     for (int i = 0; i < KU; ++i) {
@@ -966,9 +988,9 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     }
     if (wave == W - 1) {
       const uint32_t key = min(t + lane / 32, t1 - 1) * 32 + lane % 32;
-      const bool in = key < most;  // behind that there may be anything
-      re[0] = in ? kep[key] : 0;
-      re[1] = in ? vep[key] : 0;
+      re_in = key < most;  // behind that there may be anything
+      re[0] = kep[key];
+      re[1] = vep[key];
     }
   };
   auto store = [&](int half) {
@@ -994,22 +1016,48 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
       }
     }
     if (wave == W - 1) {
-      exps[half][0][lane] = re[0];
-      exps[half][1][lane] = re[1];
-      const uint64_t odd = __ballot(re[0] == kNanExp || re[1] == kNanExp || re[0] >= kBigExp);
+      const int ek = re_in ? re[0] : 0, ev = re_in ? re[1] : 0;
+      exps[half][0][lane] = ek;
+      exps[half][1][lane] = ev;
+      const uint64_t odd = __ballot(ek == kNanExp || ev == kNanExp || ek >= kBigExp);
       if (lane < 2) odds[half][lane] = (uint32_t)(odd >> (32 * lane));
     }
   };
 
   if (t0 < t1) load(t0);
-  // The rows' operands, 16 rows a wave, by way of the buffer.
+  // The rows' operands, 16 rows a wave: whole rows into LDS (read where the
+  // operands want them, a line would be fetched eight times over), from there
+  // as operands, which all the rows' waves take by way of the buffer.
+  constexpr int QR = ROW / 4, RI = 64 / QR;  // quads of a row, rows of a 64-lane access
   {
     const RowRef x = job.row(a, job.group * 32 * RW + wave * 16 + c);
+    const uint64_t at = x.bt * a.q_stride + (size_t)x.head * a.c.head_dim;
+    const int hd = (int)a.c.head_dim, d = lane % QR * 4;
+    float* own = reinterpret_cast<float*>(smem) + (size_t)wave * 16 * RS;
+    f32x4 v[16 / RI];
+#pragma unroll
+    for (int i = 0; i < 16 / RI; ++i) {
+      const float* q = a.q + shfl_u64(at, i * RI + lane / QR);
+      if (a.q_vec) {
+        v[i] = *reinterpret_cast<const f32x4*>(q + min(d, hd - 4));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = q[min(d + k, hd - 1)];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / RI; ++i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[i][k] = d + k < hd ? v[i][k] : 0.f;
+      *reinterpret_cast<f32x4*>(own + (i * RI + lane / QR) * RS + d) = v[i];
+    }
+    __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses keep their order
     RawQ<ROW> raw;
-    raw.load(a, x, g);
+    raw.from_lds(own, RS, g, c);
     f16x8 hi[KS], lo[KS];
     const float f = raw.operands(a, hi, lo);
     if (g == 0) sqf[wave * 16 + c] = f;
+    __syncthreads();
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       smem[((wave * KS + s) * 2) * 64 + lane] = __builtin_bit_cast(uint4, hi[s]);
@@ -1098,43 +1146,52 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   const uint32_t nparts = pl.prefix_splits + (pl.own_splits > 1 ? pl.own_splits : 0);
   const uint32_t at = SHARED ? job.split : pl.prefix_splits + job.split;
   auto finish = [&](f32x4* acc, float mm, float ll, const RowRef& x, int r16) {
-    if (row0 + r16 + c >= job.nrows || (!x.live && !final)) return;
     const size_t part = row_id(a, x) * nparts;
     const PartMl y = sml[row + r16];
     float top = fmaxf(mm, y.m);
     for (uint32_t e = 0; e < extra && x.live; ++e) top = fmaxf(top, ml[part + e].m);
-    auto weight_of = [&](const PartMl& z) {
+    auto weight_of = [&](const PartMl& z, float top) {
       return z.l == 0.f ? 0.f : z.l * __builtin_amdgcn_exp2f(z.m - top);
     };
-    const float f0 = weight_of({mm, ll}), f1 = weight_of(y);
+    const float f0 = weight_of({mm, ll}, top), f1 = weight_of(y, top);
     float sum = f0 + f1;
-    for (uint32_t e = 0; e < extra && x.live; ++e) sum += weight_of(ml[part + e]);
+    for (uint32_t e = 0; e < extra && x.live; ++e) sum += weight_of(ml[part + e], top);
     const float inv = x.live && sum != 0.f ? 1.f / sum : 0.f;
-    f32x4 o[DT];  // [r][j / 4]: columns (4 g + r) DT + j ..
+    float* mine = so + (size_t)(row + r16) * RS + 4 * g * DT;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int j = 0; j < DT; j += 4)
-        o[r * (DT / 4) + j / 4] =
-            f0 * inv * f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]} +
-            f1 * inv *
-                *reinterpret_cast<const f32x4*>(so + (size_t)(row + r16) * RS + (4 * g + r) * DT + j);
-    for (uint32_t e = 0; e < extra && x.live; ++e) {
-      const float f = weight_of(ml[part + e]) * inv;
+      for (int j = 0; j < DT; j += 4) {
+        f32x4* at = reinterpret_cast<f32x4*>(mine + r * DT + j);
+        *at = f0 * inv * f32x4{acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]} +
+              f1 * inv * *at;
+      }
+    __builtin_amdgcn_wave_barrier();  // a wave's LDS accesses keep their order
+    // Whole rows from here.
+    const bool there = row0 + r16 + c < job.nrows && (x.live || final);
+    const uint64_t flags = __ballot(there), lives = __ballot(x.live);
+    const uint64_t o_at = out_at(a, x);
 #pragma unroll
-      for (int k = 0; k < DT; ++k)
-        o[k] += f * *reinterpret_cast<const f32x4*>(po + (part + e) * ROW + (4 * g) * DT + 4 * k);
+    for (int i = 0; i < 16 / RI; ++i) {
+      const int r = i * RI + lane / QR, col = lane % QR * 4;
+      const size_t p = shfl_u64(part, r);
+      const uint64_t out = shfl_u64(o_at, r);
+      f32x4 o = *reinterpret_cast<const f32x4*>(so + (size_t)(rw * 32 + r16 + r) * RS + col);
+      if (extra) {
+        const float t = __shfl(top, r, 64), n = __shfl(inv, r, 64);
+        if (lives >> r & 1)
+          for (uint32_t e = 0; e < extra; ++e)
+            o += weight_of(ml[p + e], t) * n * *reinterpret_cast<const f32x4*>(po + (p + e) * ROW + col);
+      }
+      if (!(lives >> r & 1)) o = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (flags >> r & 1) {
+        if (!final)
+          *reinterpret_cast<f32x4*>(po + (p + at) * ROW + col) = o;
+        else
+          store_out(a, out, col, o);
+      }
     }
-#pragma unroll
-    for (int k = 0; k < DT; ++k) {
-      const uint32_t col = (4 * g) * DT + 4 * k;
-      if (!x.live) o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (!final)
-        *reinterpret_cast<f32x4*>(po + (part + at) * ROW + col) = o[k];
-      else
-        store_out(a, x, col, o[k]);
-    }
-    if (g == 0) {
+    if (g == 0 && there) {
       const bool some = x.live && sum != 0.f;
       if (!final)
         ml[part + at] = {some ? top : -INFINITY, some ? sum : 0.f};
@@ -1267,6 +1324,7 @@ Deal deal(uint64_t jobs, uint64_t tiles, uint32_t rt, uint32_t row, uint64_t ids
                           : rounds * (8 + (double)div_up(tiles, 2 * (uint64_t)s) * 2.1);
       if (s > 1 || joined) t += (double)ids * s * row * 8 / 4e6;
       if (s > 1 && !joined) t += 4;
+      if (w == 2 && rt <= 16) t *= 1.05;  // four waves even out a block's tail
       if (t < least) {
         least = t;
         best.splits = s;
