@@ -166,8 +166,8 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
 //
 // The exponents: a key's K scale multiplies its scores, its V scale its
 // weights.  Weights are kept at 2^(x - mt) 2^(ve - eb) with mt (per row) and
-// eb (per wave) such that the largest lies at 2^8, whole powers of two; they
-// may grow to 2^15 before mt and eb move and the accumulators are rescaled
+// eb (per wave) such that the largest lies at 2^6 (PACK: 2^3), whole powers of
+// two; they may grow to 61440 before mt and eb move and the accumulators are rescaled
 // (exactly), so most tiles neither join maxima across lanes nor rescale.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -552,11 +552,11 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       float big = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
-      over |= big > 32768.f || add[n] > 0x1p110f;
+      over |= big > 61440.f || add[n] > 0x1p110f;
     }
   }
   if (__any(over)) {
-    // New levels: the largest x + ve of a row at 2^8.  eb is 0 unless the
+    // New levels: the largest x + ve of a row at 2^6 or 2^3.  eb is 0 unless the
     // values' scales are far from 1.
     asm volatile("");
     int high = -126;
@@ -578,7 +578,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       }
       st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
-      float m1 = fmaxf(st.top_w[n] - (float)eb1 - 8.f, st.top_x[n] - 100.f);
+      float m1 = fmaxf(st.top_w[n] - (float)eb1 - (PACK ? 3.f : 6.f), st.top_x[n] - 100.f);
       if (m1 == -INFINITY) m1 = 0.f;  // no key yet
       if (!st.fresh) {
         st.l[n] *= __builtin_amdgcn_exp2f(st.mt[n] - m1);
@@ -609,14 +609,14 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     uint32_t h[4], o[4];
     st.l[n] += add[n];
     if constexpr (PACK) {
-      const uint32_t cut = c < 8 ? 0u : 0xFFFFE000u;  // hi's bits
+      const float mine = c < 8 ? 1.f : 2048.f, hi = c < 8 ? 0.f : -2048.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4; ++i) {  // w, or 2^11 (w - hi)
         const float x = w[n][2 * i], y = w[n][2 * i + 1];
+        const h2 r = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x, y));
         h[i] = __builtin_bit_cast(
-            uint32_t,
-            __builtin_amdgcn_cvt_pkrtz(x - __uint_as_float(__float_as_uint(x) & cut),
-                                       y - __uint_as_float(__float_as_uint(y) & cut)));
+            uint32_t, __builtin_amdgcn_cvt_pkrtz(fmaf(x, mine, (float)r[0] * hi),
+                                                 fmaf(y, mine, (float)r[1] * hi)));
       }
     } else {
 #pragma unroll
@@ -835,7 +835,7 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[i] = st.acc[0][j + i][r];
-        if constexpr (PACK) o[i] += dpp_f32<0x128>(o[i]);
+        if constexpr (PACK) o[i] = fmaf(dpp_f32<0x128>(o[i]), 0x1p-11f, o[i]);
         o[i] *= inv;
       }
       if (st.eb != 0) {
