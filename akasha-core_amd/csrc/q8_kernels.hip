@@ -42,101 +42,136 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t v) {
   return v;
 }
 
-// One item is one head's row of K or V: ROW / 4 lanes of four columns each.
-// Items run over heads first, so a wave reads consecutive columns.
-struct Q8Item {
-  uint32_t b, t, head;
-  bool is_v;
+// Rows in and out of the cache.  A head's row of K or V is a group of ROW / 4
+// lanes of four columns each; a block takes 1024 / ROW consecutive heads (K's, then V's) of
+// R consecutive rows of one sequence, so a thread has R loads under way and a
+// wave's are whole lines.  Bound by memory: 8 x 2040 rows of 16 heads of 128
+// (268 MB of f32 and a quarter of it in codes) move at WRITE_RATE in and
+// READ_RATE out.
+struct Q8Rows {
+  uint32_t batch, rows, stride, groups, blocks;  // groups of R rows, blocks of a row's heads
+  const uint32_t* pos;
+  const uint32_t* counts;
 };
-__device__ __forceinline__ Q8Item q8_item(uint64_t id, uint32_t rows, uint32_t kv_heads) {
-  Q8Item it;
-  it.head = (uint32_t)(id % kv_heads);
-  id /= kv_heads;
-  it.is_v = id & 1;
-  id >>= 1;
-  it.t = (uint32_t)(id % rows);
-  it.b = (uint32_t)(id / rows);
-  return it;
+struct Q8Place {
+  uint32_t b, t0, head, live;  // live: rows of the step
+  uint64_t at;                 // of row t0 in the cache
+  bool is_v, in;
+};
+template <int ROW, int R>
+__device__ __forceinline__ Q8Place q8_place(const Q8Rows& a, const Q8Cache& c) {
+  Q8Place p;
+  uint32_t id = blockIdx.x;
+  uint32_t block = 0;
+  if (a.blocks > 1) {
+    block = id % a.blocks;
+    id /= a.blocks;
+  }
+  uint32_t group = 0;
+  if (a.groups > 1) {
+    group = id % a.groups;
+    id /= a.groups;
+  }
+  p.b = id;
+  p.t0 = group * R;
+  const uint32_t item = block * (1024 / ROW) + threadIdx.x / (ROW / 4);
+  p.is_v = item >= c.kv_heads;
+  p.head = p.is_v ? item - c.kv_heads : item;
+  p.in = p.head < c.kv_heads;
+  p.live = step_rows(a.counts, p.b, a.rows);
+  p.at = (uint64_t)a.pos[p.b] + p.t0;
+  return p;
 }
 
-template <int ROW, bool VEC>
+template <int ROW, int R, bool VEC>
 __global__ __launch_bounds__(256) void k_cache_write_q8(const float* k, const float* v,
-                                                        Q8Cache c, uint32_t batch, uint32_t rows,
-                                                        uint32_t stride, const uint32_t* pos,
-                                                        const uint32_t* counts) {
-  constexpr int L = ROW / 4;
-  const int col = (threadIdx.x % L) * 4;
-  const uint64_t items = (uint64_t)batch * rows * 2 * c.kv_heads;
-  const uint64_t id = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (id >= items) return;  // whole groups of L lanes leave together
-  const Q8Item it = q8_item(id, rows, c.kv_heads);
-  const uint64_t at = (uint64_t)pos[it.b] + it.t;
-  if (it.t >= step_rows(counts, it.b, rows) || at >= c.max_rows) return;
-  const float* src = (it.is_v ? v : k) + ((size_t)it.b * rows + it.t) * stride +
-                     (size_t)it.head * c.head_dim;
-  float x[4];
-  if constexpr (VEC) {
-    const float4 f = col < (int)c.head_dim ? *reinterpret_cast<const float4*>(src + col)
-                                           : make_float4(0.f, 0.f, 0.f, 0.f);
-    x[0] = f.x;
-    x[1] = f.y;
-    x[2] = f.z;
-    x[3] = f.w;
-  } else {
+                                                        Q8Cache c, Q8Rows a) {
+  const int col = threadIdx.x % (ROW / 4) * 4;
+  const Q8Place p = q8_place<ROW, R>(a, c);
+  if (!p.in || p.t0 >= p.live || p.at >= c.max_rows) return;  // a group's lanes alike
+  const uint32_t n = (uint32_t)min<uint64_t>(min(R, (int)(p.live - p.t0)), c.max_rows - p.at);
+  const float* src = (p.is_v ? v : k) + ((size_t)p.b * a.rows + p.t0) * a.stride +
+                     (size_t)p.head * c.head_dim;
+  float x[R][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = col + i < (int)c.head_dim ? src[col + i] : 0.f;
+  for (int i = 0; i < R; ++i) {
+    const float* row = src + (size_t)min((uint32_t)i, n - 1) * a.stride;
+    if constexpr (VEC) {
+      const float4 f = *reinterpret_cast<const float4*>(row + min(col, (int)c.head_dim - 4));
+      x[i][0] = f.x;
+      x[i][1] = f.y;
+      x[i][2] = f.z;
+      x[i][3] = f.w;
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) x[i][d] = row[min(col + d, (int)c.head_dim - 1)];
+    }
   }
-  uint32_t top = 0;  // magnitudes order as their bits, infinities and NaN above all
+  const size_t row0 = ((size_t)p.b * c.kv_heads + p.head) * c.cap + p.at;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  top = group_umax<L>(top);
-  // top = 1.m * 2^(E - 127); 127 * 2^e = (127 / 64) * 2^(e + 6), and 1.m <=
-  // 127 / 64 is m <= 0x7E0000.
-  const bool bad = top >= 0x7F800000u;
-  const int e = max(-126, (int)(top >> 23) - 133 + ((top & 0x7FFFFFu) > 0x7E0000u));
-  const float inv = __int_as_float((127 - e) << 23);
-  const float most = e == 122 ? 63.f : 127.f;  // 64 * 2^122 would read back as infinity
-  uint32_t packed = 0;
-  if (!bad) {
+  for (int i = 0; i < R; ++i) {
+    uint32_t top = 0;  // magnitudes order as their bits, infinities and NaN above all
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      packed |= (uint32_t)((int)fminf(fmaxf(rintf(x[i] * inv), -most), most) & 0xFF) << (8 * i);
+    for (int d = 0; d < 4; ++d) {
+      if (col + d >= (int)c.head_dim) x[i][d] = 0.f;
+      top = max(top, __float_as_uint(x[i][d]) & 0x7FFFFFFFu);
+    }
+    top = group_umax<ROW / 4>(top);
+    // top = 1.m * 2^(E - 127); 127 * 2^e = (127 / 64) * 2^(e + 6), and 1.m <=
+    // 127 / 64 is m <= 0x7E0000.
+    const bool bad = top >= 0x7F800000u;
+    const int e = max(-126, (int)(top >> 23) - 133 + ((top & 0x7FFFFFu) > 0x7E0000u));
+    const float inv = __int_as_float((127 - e) << 23);
+    const float most = e == 122 ? 63.f : 127.f;  // 64 * 2^122 would read back as infinity
+    uint32_t packed = 0;
+    if (!bad) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        packed |= (uint32_t)((int)fminf(fmaxf(rintf(x[i][d] * inv), -most), most) & 0xFF)
+                  << (8 * d);
+    }
+    if (i < (int)n) {
+      *reinterpret_cast<uint32_t*>((p.is_v ? c.v : c.k) + (row0 + i) * ROW + col) = packed;
+      if (col == 0) (p.is_v ? c.ve : c.ke)[row0 + i] = (int8_t)(bad ? kNanExp : e);
+    }
   }
-  const size_t row = ((size_t)it.b * c.kv_heads + it.head) * c.cap + at;
-  *reinterpret_cast<uint32_t*>((it.is_v ? c.v : c.k) + row * ROW + col) = packed;
-  if (col == 0) (it.is_v ? c.ve : c.ke)[row] = (int8_t)(bad ? kNanExp : e);
 }
 
-template <int ROW, bool VEC>
-__global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, float* v,
-                                                       uint32_t batch, uint32_t rows,
-                                                       uint32_t stride, const uint32_t* pos,
-                                                       const uint32_t* counts) {
-  constexpr int L = ROW / 4;
-  const int col = (threadIdx.x % L) * 4;
-  const uint64_t items = (uint64_t)batch * rows * 2 * c.kv_heads;
-  const uint64_t id = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (id >= items || col >= (int)c.head_dim) return;
-  const Q8Item it = q8_item(id, rows, c.kv_heads);
-  float* dst = it.is_v ? v : k;
-  if (!dst) return;
-  dst += ((size_t)it.b * rows + it.t) * stride + (size_t)it.head * c.head_dim + col;
-  const uint64_t at = (uint64_t)pos[it.b] + it.t;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (it.t < step_rows(counts, it.b, rows) && at < c.max_rows) {
-    const size_t row = ((size_t)it.b * c.kv_heads + it.head) * c.cap + at;
-    const uint32_t q =
-        *reinterpret_cast<const uint32_t*>((it.is_v ? c.v : c.k) + row * ROW + col);
-    const float s = exp_value((it.is_v ? c.ve : c.ke)[row]);
+template <int ROW, int R, bool VEC>
+__global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, float* v, Q8Rows a) {
+  const int col = threadIdx.x % (ROW / 4) * 4;
+  const Q8Place p = q8_place<ROW, R>(a, c);
+  float* dst = p.is_v ? v : k;
+  if (!p.in || !dst || col >= (int)c.head_dim) return;
+  dst += ((size_t)p.b * a.rows + p.t0) * a.stride + (size_t)p.head * c.head_dim + col;
+  // Rows held, of R; the others become zero.
+  const uint32_t n = p.t0 < p.live && p.at < c.max_rows
+                         ? (uint32_t)min<uint64_t>(min(R, (int)(p.live - p.t0)), c.max_rows - p.at)
+                         : 0;
+  const size_t row0 = ((size_t)p.b * c.kv_heads + p.head) * c.cap + (n ? p.at : 0);
+  uint32_t q[R];
+  int e[R];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(q >> (8 * i)) * s;
+  for (int i = 0; i < R; ++i) {
+    const size_t row = row0 + min((uint32_t)i, n ? n - 1 : 0);
+    q[i] = *reinterpret_cast<const uint32_t*>((p.is_v ? c.v : c.k) + row * ROW + col);
+    e[i] = (p.is_v ? c.ve : c.ke)[row];
   }
-  if constexpr (VEC) {
-    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < (int)c.head_dim) dst[i] = x[i];
+  for (int i = 0; i < R; ++i) {
+    if (p.t0 + i >= a.rows) break;
+    const float s = exp_value(e[i]);
+    float x[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) x[d] = i < (int)n ? (float)(int8_t)(q[i] >> (8 * d)) * s : 0.f;
+    float* out = dst + (size_t)i * a.stride;
+    if constexpr (VEC) {
+      *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (col + d < (int)c.head_dim) out[d] = x[d];
+    }
   }
 }
 
@@ -1264,16 +1299,31 @@ bool vec4(const void* p, uint32_t stride, uint32_t head_dim) {
 
 }  // namespace
 
+namespace {
+
+// One row a thread for a decode step's, four for longer stretches.
+Q8Rows rows_of(const Q8Cache& c, uint32_t batch, uint32_t rows, uint32_t stride,
+               const uint32_t* pos, const uint32_t* counts, uint32_t r, uint64_t* blocks) {
+  Q8Rows a{batch, rows, stride, (uint32_t)div_up(rows, r),
+           (uint32_t)div_up(2 * (uint64_t)c.kv_heads, 1024 / c.row), pos, counts};
+  *blocks = (uint64_t)batch * a.groups * a.blocks;
+  return a;
+}
+
+}  // namespace
+
 hipError_t launch_cache_write_q8(const float* k, const float* v, const Q8Cache& c, uint32_t batch,
                                  uint32_t rows, uint32_t stride, const uint32_t* pos,
                                  const uint32_t* counts, hipStream_t s) {
   const bool vec = vec4(k, stride, c.head_dim) && vec4(v, stride, c.head_dim);
-  const bool wide = c.row == 128;
-  const uint64_t items = (uint64_t)batch * rows * 2 * c.kv_heads;
-  const dim3 grid((uint32_t)div_up(items, wide ? 8 : 16));
-  auto* f = wide ? (vec ? k_cache_write_q8<128, true> : k_cache_write_q8<128, false>)
-                 : (vec ? k_cache_write_q8<64, true> : k_cache_write_q8<64, false>);
-  hipLaunchKernelGGL(f, grid, dim3(256), 0, s, k, v, c, batch, rows, stride, pos, counts);
+  const bool many = rows > 1;
+  uint64_t blocks;
+  const Q8Rows a = rows_of(c, batch, rows, stride, pos, counts, many ? 4 : 1, &blocks);
+#define AKH_PICK(F, ROW)                                               \
+  (many ? (vec ? F<ROW, 4, true> : F<ROW, 4, false>)                   \
+        : (vec ? F<ROW, 1, true> : F<ROW, 1, false>))
+  auto* f = c.row == 128 ? AKH_PICK(k_cache_write_q8, 128) : AKH_PICK(k_cache_write_q8, 64);
+  hipLaunchKernelGGL(f, dim3((uint32_t)blocks), dim3(256), 0, s, k, v, c, a);
   return hipGetLastError();
 }
 
@@ -1281,12 +1331,12 @@ hipError_t launch_cache_read_q8(const Q8Cache& c, float* k, float* v, uint32_t b
                                 uint32_t rows, uint32_t stride, const uint32_t* pos,
                                 const uint32_t* counts, hipStream_t s) {
   const bool vec = (!k || vec4(k, stride, c.head_dim)) && (!v || vec4(v, stride, c.head_dim));
-  const bool wide = c.row == 128;
-  const uint64_t items = (uint64_t)batch * rows * 2 * c.kv_heads;
-  const dim3 grid((uint32_t)div_up(items, wide ? 8 : 16));
-  auto* f = wide ? (vec ? k_cache_read_q8<128, true> : k_cache_read_q8<128, false>)
-                 : (vec ? k_cache_read_q8<64, true> : k_cache_read_q8<64, false>);
-  hipLaunchKernelGGL(f, grid, dim3(256), 0, s, c, k, v, batch, rows, stride, pos, counts);
+  const bool many = rows > 1;
+  uint64_t blocks;
+  const Q8Rows a = rows_of(c, batch, rows, stride, pos, counts, many ? 4 : 1, &blocks);
+  auto* f = c.row == 128 ? AKH_PICK(k_cache_read_q8, 128) : AKH_PICK(k_cache_read_q8, 64);
+#undef AKH_PICK
+  hipLaunchKernelGGL(f, dim3((uint32_t)blocks), dim3(256), 0, s, c, k, v, a);
   return hipGetLastError();
 }
 
@@ -1308,7 +1358,7 @@ struct Deal {
   uint32_t waves, splits;
 };
 Deal deal(uint64_t jobs, uint64_t tiles, uint32_t rt, uint32_t row, uint64_t ids, bool joined) {
-  static const uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  static const uint32_t kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 21, 25, 32, 42, 51, 64};
   Deal best{rt == 32 ? 2u : rt <= 64 ? 4u : 8u, 1};
   double least = 1e30;
   for (uint32_t w = rt <= 16 ? 2 : best.waves; w <= (rt <= 16 ? 4 : best.waves); w += 2)
