@@ -97,7 +97,8 @@ __global__ __launch_bounds__(256) void k_cache_write_q8(const float* k, const fl
   for (int i = 0; i < R; ++i) {
     const float* row = src + (size_t)min((uint32_t)i, n - 1) * a.stride;
     if constexpr (VEC) {
-      const float4 f = *reinterpret_cast<const float4*>(row + min(col, (int)c.head_dim - 4));
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      const f4 f = __builtin_nontemporal_load(reinterpret_cast<const f4*>(row + min(col, (int)c.head_dim - 4)));
       x[i][0] = f.x;
       x[i][1] = f.y;
       x[i][2] = f.z;
@@ -166,7 +167,8 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
     for (int d = 0; d < 4; ++d) x[d] = i < (int)n ? (float)(int8_t)(q[i] >> (8 * d)) * s : 0.f;
     float* out = dst + (size_t)i * a.stride;
     if constexpr (VEC) {
-      *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      __builtin_nontemporal_store(f4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f4*>(out));
     } else {
 #pragma unroll
       for (int d = 0; d < 4; ++d)
