@@ -584,6 +584,7 @@ struct AttnQ8Plan {
   // Rows of a job, jobs for all rows, splits of the keys, waves of a block.
   uint32_t own_rt, own_groups, own_splits, own_waves;
   uint32_t prefix_rt, prefix_groups, prefix_splits, prefix_waves;  // splits 0: no prefix
+  bool stream;                // own codes past the caches
   size_t rows_offset, bytes;  // the workspace: maxima and sums, then rows
 };
 size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix);

@@ -264,7 +264,17 @@ struct Tile {
   uint32_t ke[2], ve[2];
 };
 
-template <int ROW>
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// STREAM: past the caches, for codes that will not be met there again.
+template <bool STREAM, class T>
+__device__ __forceinline__ T load_codes(const int8_t* p) {
+  if constexpr (STREAM)
+    return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else
+    return *reinterpret_cast<const T*>(p);
+}
+template <int ROW, bool STREAM>
 __device__ __forceinline__ void load_k(Tile<ROW>& t, const int8_t* k, const int8_t* ke,
                                        const int8_t* ve, uint32_t key0, int g, int c) {
   const int8_t* kp = k + (size_t)(key0 + c) * ROW + 16 * g;
@@ -272,12 +282,13 @@ __device__ __forceinline__ void load_k(Tile<ROW>& t, const int8_t* k, const int8
   for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
     for (int u = 0; u < ROW / 64; ++u)
-      t.k[hh][u] = *reinterpret_cast<const uint4*>(kp + hh * 16 * ROW + u * 64);
+      t.k[hh][u] = __builtin_bit_cast(
+          uint4, load_codes<STREAM, u32x4>(kp + hh * 16 * ROW + u * 64));
     t.ke[hh] = *reinterpret_cast<const uint32_t*>(ke + key0 + 16 * hh + 4 * g);
     t.ve[hh] = *reinterpret_cast<const uint32_t*>(ve + key0 + 16 * hh + 4 * g);
   }
 }
-template <int ROW>
+template <int ROW, bool STREAM>
 __device__ __forceinline__ void load_v(Tile<ROW>& t, const int8_t* v, uint32_t key0, int g,
                                        int c) {
   const int8_t* vp = v + (size_t)(key0 + 4 * g) * ROW + c * (ROW / 16);
@@ -285,9 +296,9 @@ __device__ __forceinline__ void load_v(Tile<ROW>& t, const int8_t* v, uint32_t k
   for (int i = 0; i < 8; ++i) {
     const int8_t* p = vp + ((i & 3) + (i >> 2) * 16) * ROW;
     if constexpr (ROW == 64) {
-      t.v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      t.v[i][0] = load_codes<STREAM, uint32_t>(p);
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      const u32x2 w = load_codes<STREAM, u32x2>(p);
       t.v[i][0] = w.x;
       t.v[i][1] = w.y;
     }
@@ -724,7 +735,7 @@ __device__ __forceinline__ void store_out(const AttnQ8Args& a, uint64_t at, uint
 // SHARED: the prefix's keys for the rows of all sequences, as partial results.
 // Otherwise a sequence's own keys; with one split (and the prefix's partial
 // results, where there are) the block writes the output itself.
-template <int ROW, bool PACK, int WAVES, bool SHARED>
+template <int ROW, bool PACK, int WAVES, bool SHARED, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ8Args a, AttnQ8Plan pl) {
   constexpr int KS = ROW / 32;       // MFMA steps of a score
   constexpr int DT = ROW / 16;       // MFMAs of 16 output columns
@@ -748,8 +759,8 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
   const bool early = job.splits == 1;
   if (early) {
     const uint32_t key = min((uint32_t)wave * 32, src.cap - 32);
-    load_k<ROW>(even, kp, kep, vep, key, g, c);
-    load_v<ROW>(even, vp, key, g, c);
+    load_k<ROW, STREAM>(even, kp, kep, vep, key, g, c);
+    load_v<ROW, STREAM>(even, vp, key, g, c);
   }
   // The prefix's parts of the job's rows, 64 WAVES / RT lanes to a row.
   constexpr int L = 64 * WAVES / RT;
@@ -795,12 +806,12 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
   const uint32_t t0 = min(tiles, job.split * per), t1 = min(tiles, t0 + per);
   uint32_t t = t0 + wave;
   if (!early && t < t1) {
-    load_k<ROW>(even, kp, kep, vep, t * 32, g, c);
-    load_v<ROW>(even, vp, t * 32, g, c);
+    load_k<ROW, STREAM>(even, kp, kep, vep, t * 32, g, c);
+    load_v<ROW, STREAM>(even, vp, t * 32, g, c);
   }
   if (t + WAVES < t1) {
-    load_k<ROW>(odd, kp, kep, vep, (t + WAVES) * 32, g, c);
-    load_v<ROW>(odd, vp, (t + WAVES) * 32, g, c);
+    load_k<ROW, STREAM>(odd, kp, kep, vep, (t + WAVES) * 32, g, c);
+    load_v<ROW, STREAM>(odd, vp, (t + WAVES) * 32, g, c);
   }
   __syncthreads();
   f16x8 qh[1][KS], ql[1][KS];
@@ -842,9 +853,9 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
         [&](int j) { return v_frag(&tile.v[0][j / 4], ROW / 64, j); },
         [&](int hh) { return hh ? e1 : e0; }, [&](int hh) { return hh ? f1 : f0; },
         [&]() {  // its registers take the wave's next tile but one
-          if (more) load_k<ROW>(tile, kp, kep, vep, (t + 2 * WAVES) * 32, g, c);
+          if (more) load_k<ROW, STREAM>(tile, kp, kep, vep, (t + 2 * WAVES) * 32, g, c);
         });
-    if (more) load_v<ROW>(tile, vp, (t + 2 * WAVES) * 32, g, c);
+    if (more) load_v<ROW, STREAM>(tile, vp, (t + 2 * WAVES) * 32, g, c);
     t += WAVES;
   };
   while (t < t1) {
@@ -1398,6 +1409,10 @@ AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
                       p.own_rt, a.c.row, ids, false);
   p.own_splits = d.splits;
   p.own_waves = d.waves;
+  // Caches that the 256 MB behind the L2s will not hold until they are read
+  // again: 64 sequences x 16 heads of 128, us with and without streaming:
+  // 256 rows (68 MB) 17.2 and 15.9, 512 27.9 and 30.2, 2048 88.3 and 96.7.
+  p.stream = (uint64_t)a.batch * a.c.kv_heads * a.max_len * 2 * a.c.row > (96ull << 20);
   if (prefix) {  // its parts are joined with the own rows' in any case
     p.prefix_rt = rows_per_job(all);
     p.prefix_groups = (uint32_t)div_up(all, p.prefix_rt);
@@ -1418,8 +1433,15 @@ void launch_parts(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
   const dim3 grid(SHARED ? p.prefix_groups * a.c.kv_heads * p.prefix_splits
                          : a.batch * p.own_splits * a.c.kv_heads * p.own_groups);
   const uint32_t waves = SHARED ? p.prefix_waves : p.own_waves;
-  auto* f = rt == 8    ? (waves == 2 ? k_attn_q8<ROW, true, 2, SHARED> : k_attn_q8<ROW, true, 4, SHARED>)
-            : rt == 16 ? (waves == 2 ? k_attn_q8<ROW, false, 2, SHARED> : k_attn_q8<ROW, false, 4, SHARED>)
+  auto direct = [&](auto pack) {
+    constexpr bool PACK = decltype(pack)::value;
+    if constexpr (!SHARED)
+      if (p.stream)
+        return waves == 2 ? k_attn_q8<ROW, PACK, 2, false, true> : k_attn_q8<ROW, PACK, 4, false, true>;
+    return waves == 2 ? k_attn_q8<ROW, PACK, 2, SHARED, false> : k_attn_q8<ROW, PACK, 4, SHARED, false>;
+  };
+  auto* f = rt == 8    ? direct(std::true_type{})
+            : rt == 16 ? direct(std::false_type{})
             : rt == 32 ? k_attn_q8_rows<ROW, 1, SHARED>
             : rt == 64 ? k_attn_q8_rows<ROW, 2, SHARED>
                        : k_attn_q8_rows<ROW, 4, SHARED>;
