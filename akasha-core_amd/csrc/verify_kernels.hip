@@ -2,13 +2,13 @@
 // acceptance rule on the target's and the draft's logits.
 //
 // A row's probabilities are e^((l - max) / T) / sum in f64, as the sampler's
-// are.  Three launches: k_verify_stats reduces every row in parts of kPart
-// ids (maximum, its first index, the sum relative to the part's maximum);
-// k_verify_rest, a block per sequence and part, joins the parts of the
-// sequence's rows, finds its first refused draft and sums the weights of the
-// last token's distribution in chunks of 64 ids; k_verify_pick scans those sums for
-// the chunk, and the chunk for the id, where the cumulative weight passes the
-// draw.
+// are.  Two launches.  k_verify_stats reduces every row in parts of kPart
+// ids: maximum, and the sum of weights relative to the part's maximum.  Then a
+// block per sequence and part (k_verify_pick) joins the parts of the sequence's rows, finds its
+// first refused draft and sums its part's weights of the last token's
+// distribution in chunks of 16 ids; the sequence's last block to finish walks
+// the parts' sums, the chunks' and the chunk's ids to the one where the
+// cumulative weight passes the draw.
 #include <hip/hip_runtime.h>
 
 #include "common.h"
@@ -18,15 +18,14 @@ namespace akh {
 
 namespace {
 
-constexpr int kPart = 4096;        // ids of a row that one block takes
-constexpr int kPer = kPart / 256;  // of them a thread's
-constexpr int kChunk = 64;         // ids whose weights k_verify_rest sums together
-constexpr int kChunks = kPart / kChunk;
+constexpr int kPart = 4096;          // ids of a row that one block takes
+constexpr int kPer = kPart / 256;    // of them a thread's; consecutive ones are a chunk
+constexpr int kPreload = 16;         // parts whose chunk sums are fetched before one is chosen
 
 struct PartStat {
   double sum;      // of 2^(c (l - max)), c = log2(e) / T
   float max;       // -infinity: no number in the part
-  uint32_t first;  // its first index
+  uint32_t first;  // its first index, for greedy calls
 };
 struct RowStat {
   double sum;
@@ -39,7 +38,6 @@ struct Decision {
   uint32_t row;    // of the target
   uint32_t has_q;  // a draft was refused there,
   uint32_t token;  // this one
-  uint32_t pad;
 };
 
 template <int CTRL>
@@ -97,85 +95,155 @@ __device__ __forceinline__ double wave_scan_f64(double v, int lane) {
   }
   return v;
 }
+// Where a walk over 256 threads' weights passes `point`, starting at `base`:
+// the thread, and what lies before it.  Rounding may leave none past the
+// point: the last one with weight then.
+struct Step {
+  int at;
+  double before;
+};
+struct StepShared {
+  double tot[4];
+  Step hit[4], last[4];  // of each wave; at < 0: none
+};
+__device__ Step walk(double w, double base, double point, StepShared& sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const double upto = wave_scan_f64(w, lane);
+  if (lane == 63) sh.tot[wave] = upto;
+  __syncthreads();
+  double before = base + (upto - w);
+  for (int i = 0; i < wave; ++i) before += sh.tot[i];
+  const uint64_t some = __ballot(w > 0.0);
+  const uint64_t past = __ballot(w > 0.0 && before + w > point);
+  const int hit = past ? __builtin_ctzll(past) : -1;
+  const int last = some ? 63 - __builtin_clzll(some) : -1;
+  const int id = threadIdx.x;
+  if (lane == (hit < 0 ? 0 : hit)) sh.hit[wave] = {hit < 0 ? -1 : id, before};
+  if (lane == (last < 0 ? 0 : last)) sh.last[wave] = {last < 0 ? -1 : id, before};
+  __syncthreads();
+  Step at = {0, base};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (sh.last[i].at >= 0) at = sh.last[i];
+#pragma unroll
+  for (int i = 3; i >= 0; --i)
+    if (sh.hit[i].at >= 0) at = sh.hit[i];
+  return at;
+}
 
-// Weight 2^(c (l - max)) of a logit next to its row's (or part's) maximum: a
-// power of two and the Taylor polynomial of 2^f, |f| <= 1/2, whose degree 10
-// leaves 2e-13.  The whole part n comes from the low bits of t + 1.5 2^52 and goes
-// into the exponent field as an integer, so that but for one conversion every
-// step is a full-rate f64 operation (weights below 2^-1000 are left out; that is far under the
-// sums' last bit).  A NaN, and an infinity next to an infinite maximum, has none.
-__device__ __forceinline__ double weight(float l, float max, double c) {
-  const double d = (double)l - (double)max;
-  const double m = fma(d, c, 0x1.8p52);
-  const double f = fma(d, c, -(m - 0x1.8p52));
-  double p = 7.05491162080112088e-09;
-  p = fma(p, f, 1.01780860092396960e-07);
-  p = fma(p, f, 1.32154867901443053e-06);
-  p = fma(p, f, 1.52527338040598377e-05);
-  p = fma(p, f, 1.54035303933816061e-04);
-  p = fma(p, f, 1.33335581464284411e-03);
-  p = fma(p, f, 9.61812910762847688e-03);
-  p = fma(p, f, 5.55041086648215762e-02);
-  p = fma(p, f, 2.40226506959100694e-01);
-  p = fma(p, f, 6.93147180559945286e-01);
+// 2^(n + f) from m = 1.5 2^52 + n and |f| <= 1/2: the polynomial that agrees
+// with 2^f in the ten Chebyshev points of [-1/2, 1/2] (within 4e-14 of it, and
+// 1 at 0), n put into the exponent field as an integer: so every
+// step is a full-rate f64 operation.
+__device__ __forceinline__ double power2(double m, double f) {
+  double p = 0x1.b6571de2f2351p-24;
+  p = fma(p, f, 0x1.63ef969a64d3cp-20);
+  p = fma(p, f, 0x1.ffcb76789860fp-17);
+  p = fma(p, f, 0x1.43088e257f341p-13);
+  p = fma(p, f, 0x1.5d87fe908f88ap-10);
+  p = fma(p, f, 0x1.3b2ab72b175eep-7);
+  p = fma(p, f, 0x1.c6b08d7044119p-5);
+  p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+  p = fma(p, f, 0x1.62e42fefa39f7p-1);
   p = fma(p, f, 1.0);
   const uint64_t u = __builtin_bit_cast(uint64_t, p);
   const uint32_t hi = (uint32_t)(u >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, m) << 20);
-  const double w = __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
+}
+// Weight 2^(c (l - max)) of a logit next to its row's (or part's) maximum; none
+// for a NaN, and for an infinity next to an infinite maximum.  (Weights below
+// 2^-1000 are left out, far under the sums' last bit.)
+__device__ __forceinline__ double weight(float l, float max, double c) {
+  const double d = (double)l - (double)max;
+  const double m = fma(d, c, 0x1.8p52);
+  const double w = power2(m, fma(d, c, -(m - 0x1.8p52)));
   return m > 0x1.8p52 - 1000.0 ? w : 0.0;
 }
+// The same for a sum next to which 2^-1000 is nothing: least = -1000 / c.
+__device__ __forceinline__ double weight_in_sum(float l, float max, double c, double least) {
+  const double d = fmax((double)l - (double)max, least);
+  const double m = fma(d, c, 0x1.8p52);
+  return power2(m, fma(d, c, -(m - 0x1.8p52)));
+}
 
+// Not 0 for an infinite temperature, whose weights of -infinity stay none.
 __device__ __forceinline__ double log2_scale(float temperature) {
-  return 1.4426950408889634 / (double)temperature;
+  return fmax(1.4426950408889634 / (double)temperature, 1e-60);
 }
 
 __device__ __forceinline__ uint32_t drafts_of(const VerifyArgs& a, uint32_t b) {
   return a.counts ? min(a.counts[b], a.rows) : a.rows;
 }
 
-// Rows of target first, then of draft.
-__global__ __launch_bounds__(256) void k_verify_stats(VerifyArgs a, PartStat* stats, int parts) {
-  const uint64_t row = blockIdx.x / parts;
-  const int part = blockIdx.x % parts;
-  const uint64_t trows = (uint64_t)a.batch * (a.rows + 1);
-  const bool is_target = row < trows;
-  const uint64_t r = is_target ? row : row - trows;
-  const uint32_t per = is_target ? a.rows + 1 : a.rows;
-  const uint32_t b = (uint32_t)(r / per), t = (uint32_t)(r % per);
-  const uint32_t c = drafts_of(a, b);
-  if (is_target ? t > c : t >= c) return;
-  const float* l = (is_target ? a.target : a.draft) + r * a.n;
-  float x[kPer];
-  const uint32_t id0 = part * kPart + threadIdx.x;
+// A thread's ids of a part, 256 apart; NaN past the row's end.
+__device__ __forceinline__ void load_part(const float* row, uint32_t n, int part, float* x) {
+  const uint32_t left = n - (uint32_t)part * kPart;
+  const uint32_t here = min(left, (uint32_t)kPart);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float*>(row + (size_t)part * kPart), (short)0, here * 4, 0x00020000);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = l[min(id0 + i * 256, a.n - 1)];
+  for (int i = 0; i < kPer; ++i)
+    x[i] = __builtin_bit_cast(
+        float, __builtin_amdgcn_raw_buffer_load_b32(rs, threadIdx.x * 4, i * 1024, 0));
+  if (here < kPart) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = id0 + i * 256 < a.n ? x[i] : NAN;
-  float best = -INFINITY;
-  uint32_t first = 0xFFFFFFFFu;
-#pragma unroll
-  for (int i = kPer - 1; i >= 0; --i)
-    if (x[i] >= best) {
-      best = x[i];
-      first = id0 + i * 256;
-    }
-  block_amax256(best, first);
-  double sum = 0.0;
-  if (a.temperature > 0.f) {
-    const double c2 = log2_scale(a.temperature);
-    __shared__ double red[4];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += weight(x[i], best, c2);
-    sum = block_sum_f64(sum, red);
+    for (int i = 0; i < kPer; ++i)
+      if (i * 256 + threadIdx.x >= here) x[i] = NAN;
   }
-  if (threadIdx.x == 0) stats[blockIdx.x] = {sum, best, first};
 }
 
-// Joins a row's parts, 16 lanes to a row (all of them get it); mine: the
-// lane's own part, or one without a number.
+// Rows of target first, then of draft.  32 sequences of 0 to 7 drafts over
+// 50257 ids (43 to 51 MB of live rows) take 16 to 17 us, 3 TB/s: the f64
+// arithmetic, 16 operations an id, is as long as the reads.  (With the first
+// maximum's index kept for every call and compares in place of the clamped exponent
+// it was 40 instructions an id and 22 us.)
+__global__ __launch_bounds__(256) void k_verify_stats(VerifyArgs a, PartStat* stats, int* done,
+                                                      int parts) {
+  const uint32_t row = blockIdx.x / parts;
+  const int part = blockIdx.x - row * parts;
+  const uint32_t trows = a.batch * (a.rows + 1);
+  const bool is_target = row < trows;
+  const uint32_t r = is_target ? row : row - trows;
+  const uint32_t per = is_target ? a.rows + 1 : a.rows;
+  const uint32_t b = r / per, t = r - b * per;
+  if (is_target && t == 0 && part == 0 && threadIdx.x == 0) done[b] = 0;  // for k_verify_pick
+  const uint32_t c = drafts_of(a, b);
+  if (is_target ? t > c : t >= c) return;
+  float x[kPer];
+  load_part((is_target ? a.target : a.draft) + (size_t)r * a.n, a.n, part, x);
+  if (!(a.temperature > 0.f)) {
+    float best = -INFINITY;
+    uint32_t first = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i)
+      if (x[i] >= best) {
+        best = x[i];
+        first = part * kPart + i * 256 + threadIdx.x;
+      }
+    block_amax256(best, first);
+    if (threadIdx.x == 0) stats[blockIdx.x] = {0.0, best, first};
+    return;
+  }
+  __shared__ float red_f[4];
+  __shared__ double red_d[4];
+  float best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) best = fmaxf(best, x[i]);
+  best = block_max256(best, red_f);
+  const double c2 = log2_scale(a.temperature), least = -1000.0 / c2;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += weight_in_sum(x[i], best, c2, least);
+  sum = block_sum_f64(sum, red_d);
+  if (threadIdx.x == 0)
+    stats[blockIdx.x] = {fabsf(best) < INFINITY ? sum : 0.0, best, 0xFFFFFFFFu};
+}
+
 __device__ __forceinline__ PartStat own_part(const PartStat* s, int parts, int lane) {
   return s[min(lane, parts - 1)];
 }
+// Joins a row's parts, 16 lanes to a row (all of them get it); mine: the
+// lane's first part.
 __device__ __forceinline__ RowStat join16(const PartStat* s, PartStat mine, int parts, double c,
                                           int lane) {
   if (lane >= parts) mine = {0.0, -INFINITY, 0xFFFFFFFFu};
@@ -199,49 +267,65 @@ __device__ __forceinline__ double prob(float l, const RowStat& s, double c) {
   return s.sum > 0.0 ? weight(l, s.max, c) / s.sum : 0.0;
 }
 
-// What an id's weight for the last token is made of: its logits.
-struct IdLogits {
-  float p, q;  // q: 1 or 0 for drafts without logits
-};
-__device__ __forceinline__ IdLogits id_logits(const VerifyArgs& a, const Decision& d, uint32_t b,
-                                              uint32_t id, bool less_q) {
-  const uint32_t at = min(id, a.n - 1);
-  const size_t row = (size_t)b * a.rows + d.row;
-  IdLogits x{a.target[(row + b) * a.n + at], 0.f};
-  if (less_q) x.q = a.draft ? a.draft[row * a.n + at] : (d.token == id ? 1.f : 0.f);
-  if (id >= a.n) x.p = NAN;
-  return x;
-}
-// p, less q where a draft was refused; nothing past the row's end.
-__device__ __forceinline__ double id_weight(const VerifyArgs& a, const Decision& d, IdLogits x,
-                                            double c, double inv_p, double inv_q, bool less_q) {
-  const double p = weight(x.p, d.p.max, c) * inv_p;
-  if (!less_q) return p;
-  const double q = a.draft ? weight(x.q, d.q.max, c) * inv_q : (double)x.q;
-  return fmax(p - q, 0.0);
-}
-__device__ __forceinline__ double inverse(double x) { return x > 0.0 ? 1.0 / x : 0.0; }
+// What an id's weight for the last token is made of.
+struct Draw {
+  const float* p;  // the target's row
+  const float* q;  // the draft's, or null
+  uint32_t token;  // the draft without a distribution, or no id
+  float pm, qm;
+  double c, inv_p, inv_q;
+  bool less_q;
 
+  // q without logits: 1 or 0.
+  __device__ __forceinline__ double of(float lp, float lq) const {
+    const double w = weight(lp, pm, c) * inv_p;
+    if (!less_q) return w;
+    return fmax(w - (q ? weight(lq, qm, c) * inv_q : (double)lq), 0.0);
+  }
+  __device__ __forceinline__ double of_id(uint32_t id, uint32_t n) const {
+    if (id >= n) return 0.0;
+    return of(p[id], !less_q ? 0.f : q ? q[id] : token == id ? 1.f : 0.f);
+  }
+};
+
+__device__ __forceinline__ double agent_load(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void agent_store(double* p, double x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Slot of an id's logit in a part's LDS copy: four words apart every sixteen,
+// so that threads reading sixteen in a row keep off each other's banks.
+__device__ __forceinline__ int slot(int i) { return i + (i >> 4) * 4; }
+
+// A chain of loads and short scans, each waiting for the one before it: 11 us
+// for one sequence, 15 us for 32 (two rows of 50257 ids each, 13 MB, and the
+// rest of the chip idle).  As a launch of its own after one that sums the chunks it was
+// 8 us on top of 16; the hand-off to the last block costs 1.4.
 // A block per sequence and part (one part when greedy).  Every block joins
 // the sequence's rows, 16 at a time with 16 lanes each, up to the first refused draft.
-__global__ __launch_bounds__(256) void k_verify_rest(VerifyArgs a, const PartStat* stats,
-                                                     double* sums, Decision* decisions,
+// The sums are written through to device scope and counted there; the count
+// starts at zero by k_verify_stats.
+__global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartStat* stats,
+                                                     double* sums, double* totals, int* done,
                                                      int parts) {
   const bool greedy = !(a.temperature > 0.f);
   const int per = greedy ? 1 : parts;  // blocks of a sequence: no weights to sum when greedy
   const uint32_t b = blockIdx.x / per;
-  const int part = blockIdx.x % per;
+  const int part = blockIdx.x - b * per;
   const uint32_t c = drafts_of(a, b);
   const double c2 = greedy ? 1.0 : log2_scale(a.temperature);
   const uint64_t trow = (uint64_t)b * (a.rows + 1);
   const uint64_t qrow = (uint64_t)a.batch * (a.rows + 1) + (uint64_t)b * a.rows;
   const int group = threadIdx.x >> 4, lane16 = threadIdx.x & 15;
+  const double last_u = greedy ? 0.0 : a.uniforms[trow + a.rows];
   __shared__ uint32_t refused;
   __shared__ Decision dec;
-  if (threadIdx.x == 0) refused = c;
   bool decided = false;
   // Past the refused row only the chances are wanted, of the first part's block.
-  for (uint32_t t0 = 0; t0 <= c; t0 += 16) {
+  uint32_t t0 = 0;
+  do {
     const uint32_t t = t0 + group;
     // Loaded whether or not the row is live (inside the buffers either way), so that
     // counts, tokens and the parts arrive together.
@@ -250,14 +334,15 @@ __global__ __launch_bounds__(256) void k_verify_rest(VerifyArgs a, const PartSta
     const PartStat* sp = stats + (trow + tr) * parts;
     const PartStat* sq = stats + (qrow + td) * parts;
     const PartStat mp = own_part(sp, parts, lane16);
-    const bool two = a.draft != nullptr;
+    const bool two = a.draft != nullptr && a.rows;
     const PartStat mq = two ? own_part(sq, parts, lane16) : PartStat{0.0, -INFINITY, 0};
-    const double u = greedy ? 0.0 : a.uniforms[(size_t)b * (a.rows + 1) + tr];
+    const double u = greedy ? 0.0 : a.uniforms[trow + tr];
     const uint32_t xi = x < a.n ? x : 0;
     const float lp = a.target[(trow + tr) * a.n + xi];
     const float lq = two ? a.draft[((size_t)b * a.rows + td) * a.n + xi] : 0.f;
     RowStat p{}, q{};
     bool ok = true;
+    if (t0 == 0 && threadIdx.x == 0) refused = c;
     __syncthreads();
     if (t <= c) {
       p = join16(sp, mp, parts, c2, lane16);
@@ -292,113 +377,127 @@ __global__ __launch_bounds__(256) void k_verify_rest(VerifyArgs a, const PartSta
       decided = true;
       if (part != 0) break;
     }
-  }
+    t0 += 16;
+  } while (t0 <= c);
   __syncthreads();
+  const Decision d = dec;
   if (part == 0) {
-    const uint32_t r = dec.row;
     for (uint32_t t = threadIdx.x; t <= a.rows; t += 256) {
-      if (t != r) a.out_tokens[trow + t] = t < r ? a.tokens[(size_t)b * a.rows + t] : 0xFFFFFFFFu;
+      if (t != d.row)
+        a.out_tokens[trow + t] = t < d.row ? a.tokens[(size_t)b * a.rows + t] : 0xFFFFFFFFu;
       if (t >= c && t < a.rows && a.chance) a.chance[(size_t)b * a.rows + t] = 0.f;
     }
     if (threadIdx.x == 0) {
-      a.out_counts[b] = r + 1;
-      if (greedy) a.out_tokens[trow + r] = dec.p.first;
-      decisions[b] = dec;
+      a.out_counts[b] = d.row + 1;
+      if (greedy) a.out_tokens[trow + d.row] = d.p.first;
     }
   }
   if (greedy) return;
-  const Decision d = dec;
-  const double inv_p = inverse(d.p.sum), inv_q = inverse(d.q.sum);
-  const int wave = threadIdx.x >> 6;
-  double* s = sums + ((size_t)b * parts + part) * kChunks;
-  IdLogits x[kPer];
-  const uint32_t id0 = part * kPart + threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) x[i] = id_logits(a, d, b, id0 + i * 256, d.has_q);
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const double w = wave_sum_f64(id_weight(a, d, x[i], c2, inv_p, inv_q, d.has_q));
-    if ((threadIdx.x & 63) == 0) s[i * 4 + wave] = w;
-  }
-}
 
-// A block per sequence: the chunk of ids in which the cumulative weight
-// passes the draw, then the id in it.
-__global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, double* sums,
-                                                     const Decision* decisions, int parts) {
-  const uint32_t b = blockIdx.x;
-  const Decision d = decisions[b];
-  const double c2 = log2_scale(a.temperature);
-  const double inv_p = inverse(d.p.sum), inv_q = inverse(d.q.sum);
-  const double u = a.uniforms[(size_t)b * (a.rows + 1) + a.rows];
-  uint32_t* out = a.out_tokens + (size_t)b * (a.rows + 1) + d.row;
-  double* s = sums + (size_t)b * parts * kChunks;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = parts * kChunks, per = n / 256 + (n % 256 != 0);
-  const int i0 = min(n, (int)threadIdx.x * per), i1 = min(n, i0 + per);
-  __shared__ double tot[4];
-  __shared__ int hit, last;
-  __shared__ double base;
-  bool less_q = d.has_q;
-  double before = 0.0, total = 0.0;
-  for (int round = 0; round < 2; ++round) {
+  Draw w;
+  w.p = a.target + (trow + d.row) * a.n;
+  w.less_q = d.has_q;
+  w.q = d.has_q && a.draft ? a.draft + ((size_t)b * a.rows + d.row) * a.n : nullptr;
+  w.token = d.token;
+  w.pm = d.p.max;
+  w.qm = d.q.max;
+  w.c = c2;
+  w.inv_p = d.p.sum > 0.0 ? 1.0 / d.p.sum : 0.0;
+  w.inv_q = d.q.sum > 0.0 ? 1.0 / d.q.sum : 0.0;
+  // The part's logits, by way of LDS into threads of sixteen consecutive ids.
+  constexpr int kSlots = kPart + kPart / 4;
+  __shared__ __attribute__((aligned(16))) float xs[2][kSlots];
+  __shared__ double red[4];
+  {
+    float x[kPer], y[kPer];
+    load_part(w.p, a.n, part, x);
+    if (w.q) load_part(w.q, a.n, part, y);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = i * 256 + threadIdx.x;
+      xs[0][slot(id)] = x[i];
+      if (w.q) xs[1][slot(id)] = y[i];
+    }
+    __syncthreads();
     double own = 0.0;
-    for (int i = i0; i < i1; ++i) own += s[i];
-    const double upto = wave_scan_f64(own, lane);
-    if (lane == 63) tot[wave] = upto;
-    if (threadIdx.x == 0) {
-      hit = n;
-      last = -1;
-    }
-    __syncthreads();
-    before = upto - own;
-    for (int w = 0; w < wave; ++w) before += tot[w];
-    total = ((tot[0] + tot[1]) + tot[2]) + tot[3];
-    if (total > 0.0 || !less_q) break;
-    // Nothing of p exceeds q: p itself, whose sums are made here.
-    less_q = false;
-    for (int i = threadIdx.x; i < n; i += 256) {
-      double w = 0.0;
-      for (int k = 0; k < kChunk; ++k) {
-        const uint32_t id = (uint32_t)i * kChunk + k;
-        w += id_weight(a, d, id_logits(a, d, b, id, false), c2, inv_p, inv_q, false);
+    const uint32_t id0 = part * kPart + threadIdx.x * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+      const float4 lp = *reinterpret_cast<const float4*>(&xs[0][slot(threadIdx.x * kPer) + i]);
+      float4 lq = w.q ? *reinterpret_cast<const float4*>(&xs[1][slot(threadIdx.x * kPer) + i])
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (w.less_q && !w.q) {
+        lq.x = w.token == id0 + i ? 1.f : 0.f;
+        lq.y = w.token == id0 + i + 1 ? 1.f : 0.f;
+        lq.z = w.token == id0 + i + 2 ? 1.f : 0.f;
+        lq.w = w.token == id0 + i + 3 ? 1.f : 0.f;
       }
-      s[i] = w;
+      own += (w.of(lp.x, lq.x) + w.of(lp.y, lq.y)) + (w.of(lp.z, lq.z) + w.of(lp.w, lq.w));
     }
-    __syncthreads();
+    agent_store(sums + ((size_t)b * parts + part) * 256 + threadIdx.x, own);
+    const double total = block_sum_f64(own, red);
+    if (threadIdx.x == 0) agent_store(totals + (size_t)b * parts + part, total);
   }
-  if (!(total > 0.0)) {
-    if (threadIdx.x == 0) *out = d.p.first;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  __shared__ bool last_block;
+  if (threadIdx.x == 0)
+    last_block = __hip_atomic_fetch_add(done + b, 1, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+  __syncthreads();
+  if (!last_block) return;
+
+  double* s = sums + (size_t)b * parts * 256 + threadIdx.x;
+  uint32_t* out = a.out_tokens + trow + d.row;
+  double v[kPreload];
+#pragma unroll
+  for (int i = 0; i < kPreload; ++i) v[i] = i < parts ? agent_load(s + (size_t)i * 256) : 0.0;
+  double mine = (int)threadIdx.x < parts ? agent_load(totals + (size_t)b * parts + threadIdx.x) : 0.0;
+  double total = block_sum_f64(mine, red);
+  bool fetched = parts <= kPreload;
+  if (!(total > 0.0) && w.less_q) {
+    // Nothing of p exceeds q: p itself, whose sums are made here.
+    w.less_q = false;
+    for (int i = 0; i < parts; ++i) {
+      double own = 0.0;
+      for (int k = 0; k < kPer; ++k)
+        own += w.of_id((uint32_t)i * kPart + threadIdx.x * kPer + k, a.n);
+      agent_store(s + (size_t)i * 256, own);
+      const double sum = block_sum_f64(own, red);
+      if ((int)threadIdx.x == i) mine = sum;
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    total = block_sum_f64(mine, red);
+    fetched = false;
+  }
+  if (!(total > 0.0)) {  // no weight at all: the row's first maximum
+    __syncthreads();
+    if (threadIdx.x == 0) refused = a.n;
+    __syncthreads();
+    for (uint32_t id = threadIdx.x; id < a.n; id += 256)
+      if (w.p[id] == w.pm) {
+        atomicMin(&refused, id);
+        break;
+      }
+    __syncthreads();
+    if (threadIdx.x == 0) *out = refused < a.n ? refused : 0;
     return;
   }
-  const double point = u * total;
-  double cum = before;
-  int mine = n, weighty = -1;
-  for (int i = i0; i < i1; ++i) {
-    const double w = s[i];
-    cum += w;
-    if (w > 0.0) {
-      weighty = i;
-      if (cum > point && mine == n) mine = i;
-    }
+  __shared__ StepShared sh;
+  const double point = last_u * total;
+  const Step at = walk(mine, 0.0, point, sh);
+  double chunk = 0.0;
+  if (fetched) {
+#pragma unroll
+    for (int i = 0; i < kPreload; ++i) chunk = i == at.at ? v[i] : chunk;
+  } else {
+    chunk = agent_load(s + (size_t)at.at * 256);
   }
-  if (mine < n) atomicMin(&hit, mine);
-  if (weighty >= 0) atomicMax(&last, weighty);
-  __syncthreads();
-  const int chunk = hit < n ? hit : last;  // rounding may leave none past the point
-  if (chunk >= i0 && chunk < i1) {
-    cum = before;
-    for (int i = i0; i < chunk; ++i) cum += s[i];
-    base = cum;
-  }
-  __syncthreads();
-  if (wave) return;
-  const uint32_t id = (uint32_t)chunk * kChunk + lane;
-  const double w = id_weight(a, d, id_logits(a, d, b, id, less_q), c2, inv_p, inv_q, less_q);
-  const double upto = base + wave_scan_f64(w, lane);
-  const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && upto > point);
-  const int k = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some);
-  if (lane == 0) *out = (uint32_t)chunk * kChunk + k;
+  const Step in = walk(chunk, at.before, point, sh);
+  const uint32_t id0 = (uint32_t)at.at * kPart + in.at * kPer;
+  const Step id = walk(threadIdx.x < kPer ? w.of_id(id0 + threadIdx.x, a.n) : 0.0, in.before,
+                       point, sh);
+  if (threadIdx.x == 0) *out = id0 + id.at;
 }
 
 int parts_of(uint32_t n) { return (int)((n + kPart - 1) / kPart); }
@@ -412,21 +511,20 @@ uint64_t verify_blocks(uint32_t batch, uint32_t rows, uint32_t n) {
 
 size_t verify_workspace_bytes(uint32_t batch, uint32_t rows, uint32_t n) {
   return verify_blocks(batch, rows, n) * sizeof(PartStat) +
-         (size_t)batch * (parts_of(n) * kChunks * sizeof(double) + sizeof(Decision));
+         (size_t)batch * (parts_of(n) * 257 * sizeof(double) + sizeof(int));
 }
 
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
   const int parts = parts_of(a.n);
   PartStat* stats = static_cast<PartStat*>(a.ws);
   double* sums = reinterpret_cast<double*>(stats + verify_blocks(a.batch, a.rows, a.n));
-  Decision* dec = reinterpret_cast<Decision*>(sums + (size_t)a.batch * parts * kChunks);
+  double* totals = sums + (size_t)a.batch * parts * 256;
+  int* done = reinterpret_cast<int*>(totals + (size_t)a.batch * parts);
   const uint64_t rows = a.draft ? stat_rows(a.batch, a.rows) : (uint64_t)a.batch * (a.rows + 1);
   hipLaunchKernelGGL(k_verify_stats, dim3((uint32_t)(rows * parts)), dim3(256), 0, s, a, stats,
-                     parts);
-  hipLaunchKernelGGL(k_verify_rest, dim3((uint32_t)(a.temperature > 0.f ? a.batch * parts : a.batch)),
-                     dim3(256), 0, s, a, stats, sums, dec, parts);
-  if (a.temperature > 0.f)
-    hipLaunchKernelGGL(k_verify_pick, dim3(a.batch), dim3(256), 0, s, a, sums, dec, parts);
+                     done, parts);
+  hipLaunchKernelGGL(k_verify_pick, dim3(a.temperature > 0.f ? a.batch * parts : a.batch),
+                     dim3(256), 0, s, a, stats, sums, totals, done, parts);
   return hipGetLastError();
 }
 

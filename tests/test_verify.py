@@ -203,6 +203,19 @@ def test_rows_of_nan_and_infinities(backend, pkg, temperature):
 
 
 @gpu
+@pytest.mark.parametrize("temperature", [np.inf, 3e38, 1e-38, 1e-45])
+def test_temperatures_at_the_ends(backend, pkg, temperature):
+    # Hot: all numbers above -infinity alike; cold: the maxima alone.
+    rng = np.random.default_rng(12)
+    target, draft, tokens, u = make(rng, 6, 3, 5000)
+    target[:3, :, 1::2] = -np.inf
+    draft[3:, :, ::3] = np.nan
+    target[:, :, [7, 4999]] = target.max()
+    check(pkg, backend, target, draft, tokens, temperature, u, None)
+    check(pkg, backend, target, None, tokens, temperature, u, None)
+
+
+@gpu
 def test_without_drafts_it_samples(backend, pkg, ora):
     # rows = 0 (or counts 0) draws from the row itself, as the sampler's
     # temperature does, though not in the sampler's order of ids.
