@@ -552,8 +552,9 @@ struct Q8Cache {
   int8_t* ve;
   uint32_t slots, max_rows, cap, row, kv_heads, head_dim;
 };
-// A launch's grid holds at most this many blocks.
-constexpr uint64_t kMaxBlocks = 0x7FFFFFFF;
+// Blocks of 256 threads that a launch may have (its threads are counted in 32 bits).
+constexpr uint64_t kMaxBlocks = 0xFFFFFF;
+uint64_t cache_q8_blocks(const Q8Cache& c, uint32_t batch, uint32_t rows);
 hipError_t launch_cache_write_q8(const float* k, const float* v, const Q8Cache& c, uint32_t batch,
                                  uint32_t rows, uint32_t stride, const uint32_t* pos,
                                  const uint32_t* counts, hipStream_t s);

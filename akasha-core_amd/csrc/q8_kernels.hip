@@ -45,9 +45,10 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t v) {
 // Rows in and out of the cache.  A head's row of K or V is a group of ROW / 4
 // lanes of four columns each; a block takes 1024 / ROW consecutive heads (K's, then V's) of
 // R consecutive rows of one sequence, so a thread has R loads under way and a
-// wave's are whole lines.  Bound by memory: 8 x 2040 rows of 16 heads of 128
-// (268 MB of f32 and a quarter of it in codes) move at WRITE_RATE in and
-// READ_RATE out.
+// wave's are whole lines.  Bound by memory: of 8 x 2040 rows of 16 heads of 128
+// with 10987 rows live (180 MB of f32 and 45 of codes; the read fills all 267 MB)
+// the write takes 43 us and the read 45.  Both together were 145 us with a row a
+// thread, 114 with four, and are 88 with f32 past the caches.
 struct Q8Rows {
   uint32_t batch, rows, stride, groups, blocks;  // groups of R rows, blocks of a row's heads
   const uint32_t* pos;
@@ -820,7 +821,8 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     qh[0][s] = f16x8_of(sq[0][s][lane]);
     if constexpr (!PACK) ql[0][s] = f16x8_of(sq[1][s][lane]);
   }
-  const float qf = sqf[c];
+  // Rows that are not there weigh every key alike, so that their scores move no levels.
+  const float qf = ref.live ? sqf[c] : 0.f;
   RowsState<ROW, 1> st;
   st.init();
   auto step = [&](Tile<ROW>& tile) {
@@ -1121,7 +1123,7 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   for (int n = 0; n < NT; ++n) {
     ref[n] = job.row(a, row0 + n * 16 + c);
     limit[n] = ref[n].limit;
-    qf[n] = sqf[rw * 32 + n * 16 + c];
+    qf[n] = ref[n].live ? sqf[rw * 32 + n * 16 + c] : 0.f;  // as in k_attn_q8
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qh[n][s] = f16x8_of(smem[(((rw * 2 + n) * KS + s) * 2) * 64 + lane]);
@@ -1284,7 +1286,6 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan p
     const float inv = total == 0.f ? 0.f : 1.f / total;
     f[0] *= inv;
     f[1] *= inv;
-#pragma unroll 8
     for (int p = wave; p < n; p += 4) {
       const float w = __shfl(p < 64 ? f[0] : f[1], p & 63, 64);
 #pragma unroll
@@ -1324,6 +1325,12 @@ Q8Rows rows_of(const Q8Cache& c, uint32_t batch, uint32_t rows, uint32_t stride,
 }
 
 }  // namespace
+
+uint64_t cache_q8_blocks(const Q8Cache& c, uint32_t batch, uint32_t rows) {
+  uint64_t blocks;
+  rows_of(c, batch, rows, 0, nullptr, nullptr, rows > 1 ? 4 : 1, &blocks);
+  return blocks;
+}
 
 hipError_t launch_cache_write_q8(const float* k, const float* v, const Q8Cache& c, uint32_t batch,
                                  uint32_t rows, uint32_t stride, const uint32_t* pos,
@@ -1376,7 +1383,8 @@ Deal deal(uint64_t jobs, uint64_t tiles, uint32_t rt, uint32_t row, uint64_t ids
   double least = 1e30;
   for (uint32_t w = rt <= 16 ? 2 : best.waves; w <= (rt <= 16 ? 4 : best.waves); w += 2)
     for (uint32_t s : kSplits) {
-      if (s > kAttnMaxSplits || (s > 1 && tiles / s < (rt <= 16 ? 2 * w : 4))) break;
+      if (s > kAttnMaxSplits || jobs * s * w > kMaxBlocks * 4 ||
+          (s > 1 && tiles / s < (rt <= 16 ? 2 * w : 4))) break;
       const double cap = (double)kCus * (rt > 16 ? (rt == 32 && row == 128 ? 4 : 8)
                                                  : row == 64 ? 12 : 8);
       const double full = (double)(jobs * s * w) / cap;

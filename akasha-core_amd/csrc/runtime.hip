@@ -717,7 +717,8 @@ akh_status q8_rows_args(const akh_q8_cache& cache, uint32_t batch, uint32_t rows
   CHECK_ARG(batch <= c->slots, "q8 cache rows: batch exceeds the cache's slots");
   CHECK_ARG((uint64_t)stride >= (uint64_t)c->kv_heads * c->head_dim,
             "q8 cache rows: row stride below kv_heads * head_dim");
-  CHECK_ARG((unsigned __int128)batch * rows * 2 * c->kv_heads <= kMaxBlocks,
+  CHECK_ARG((uint64_t)batch * rows <= kMaxBlocks * 4 &&
+                cache_q8_blocks(*c, batch, rows) <= kMaxBlocks,
             "q8 cache rows: too many rows for one call");
   return AKH_OK;
 }
@@ -737,8 +738,8 @@ akh_status attn_q8_args(const akh_attn_q8& s, const akh_q8_cache& cache,
   CHECK_ARG(s.q_stride >= width && s.out_stride >= width,
             "q8 attention: row stride below heads * head_dim");
   CHECK_ARG(isfinite(s.scale), "q8 attention: scale must be finite");
-  CHECK_ARG((unsigned __int128)s.batch * s.rows * s.heads <= (1u << 24),
-            "q8 attention: batch * rows * heads exceeds 2^24");
+  CHECK_ARG((unsigned __int128)s.batch * s.rows * s.heads <= kMaxBlocks,
+            "q8 attention: batch * rows * heads must be below 2^24");
   a->batch = s.batch;
   a->rows = s.rows;
   a->heads = s.heads;

@@ -177,15 +177,14 @@ __device__ __forceinline__ uint32_t drafts_of(const VerifyArgs& a, uint32_t b) {
 
 // A thread's ids of a part, 256 apart; NaN past the row's end.
 __device__ __forceinline__ void load_part(const float* row, uint32_t n, int part, float* x) {
-  const uint32_t left = n - (uint32_t)part * kPart;
-  const uint32_t here = min(left, (uint32_t)kPart);
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float*>(row + (size_t)part * kPart), (short)0, here * 4, 0x00020000);
+  const uint32_t here = min(n - (uint32_t)part * kPart, (uint32_t)kPart);
+  const float* p = row + (size_t)part * kPart;
+  if (here == kPart) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    x[i] = __builtin_bit_cast(
-        float, __builtin_amdgcn_raw_buffer_load_b32(rs, threadIdx.x * 4, i * 1024, 0));
-  if (here < kPart) {
+    for (int i = 0; i < kPer; ++i) x[i] = p[i * 256 + threadIdx.x];
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = p[min(i * 256 + threadIdx.x, here - 1)];
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (i * 256 + threadIdx.x >= here) x[i] = NAN;

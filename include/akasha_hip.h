@@ -272,7 +272,11 @@ akh_status akh_sample_rows_noalloc(akh_backend* be, const float* logits, uint32_
  * pos, counts and prefix_len are device arrays read when the kernels run, so
  * a captured graph follows them as it follows metas.  Every call is queued on
  * the backend's stream and allocates nothing.  Work for zero sequences or
- * rows is AKH_OK and does nothing.
+ * rows is AKH_OK and does nothing.  A call of more work than one grid of 2^24 - 1
+ * blocks holds is refused (AKH_E_INVALID): attention of 2^24 query rows times
+ * heads, cache rows of that many times 16 heads (8 above head_dim 64) by four
+ * rows, drafts of that many logit rows times 4096 ids.  Buffers that a call writes
+ * may not overlap those that it reads.
  *
  * A workspace is device memory of the size its *_workspace function tells,
  * aligned to 16 bytes, that a call uses until its kernels have run: calls on
@@ -329,17 +333,19 @@ akh_status akh_attn_q8_workspace(const akh_attn_q8* shape, const akh_q8_cache* c
 /* out[b, t, h] = sum_j softmax_j(scale q[b, t, h] . k_j) v_j over the cache
  * rows j <= pos[b] + t, j < max_rows of slot b, and lse[b, t, h] ([batch,
  * rows, heads], may be NULL) = ln sum_j exp(scale q . k_j).  Rows t >=
- * counts[b] get zeros and -infinity.  Products in two fp16 terms of q and of
- * the softmax weights with the exact codes, sums in f32: the accuracy of f32
- * arithmetic on the cache's values.  NaN and infinities in q and NaN rows of
- * the cache make the heads that use them NaN.  out may not overlap q. */
+ * counts[b] get zeros and -infinity, and what q holds in them is not looked
+ * at.  Products in two fp16 terms (22 bits) of q and of the softmax weights
+ * with the exact codes, sums in f32: the accuracy of f32 arithmetic on the
+ * cache's values.  Next to the key that adds most to a row, what a key adds is kept to
+ * 2^-31 of that.  NaN and infinities in q and NaN rows of the cache make the
+ * heads that use them NaN. */
 akh_status akh_attn_cached_q8(akh_backend* be, const float* q, akh_q8_cache cache, float* out,
                               float* lse, akh_attn_q8 shape, const uint32_t* pos,
                               const uint32_t* counts, void* workspace, size_t workspace_bytes);
 /* akh_attn_cached_q8 where every sequence has the rows j < prefix_len[0] (at
  * most max_rows) of slot 0 of `prefix` before its own: a prompt that the
- * batch shares is stored once, and read once for all of a kv head's query rows
- * (32 at a time).  prefix has the cache's kv_heads and head_dim. */
+ * batch shares is stored once, and read once for up to 128 query rows of a kv
+ * head.  prefix has the cache's kv_heads and head_dim. */
 akh_status akh_attn_prefix_q8(akh_backend* be, const float* q, akh_q8_cache prefix,
                               const uint32_t* prefix_len, akh_q8_cache cache, float* out,
                               float* lse, akh_attn_q8 shape, const uint32_t* pos,

@@ -385,6 +385,80 @@ def test_attention_of_uneven_magnitudes(backend, pkg, hd):
 
 
 @gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd", [(1, 8, 1, 128), (5, 4, 2, 64), (16, 2, 1, 64),
+                                               (24, 2, 1, 100), (40, 3, 1, 64), (33, 8, 2, 128)])
+def test_attention_of_uneven_rows(backend, pkg, rows, heads, kvh, hd):
+    # The same in every tile of rows: levels that rise along the keys, values'
+    # scales far from 1 in one head, K's beyond 2^90 in another sequence.
+    rng = np.random.default_rng(rows * heads)
+    batch, n, ahead = 3, 333, 150
+    k, v = (rng.standard_normal((batch, n, kvh, hd)) for _ in range(2))
+    q = rng.standard_normal((batch, rows, heads, hd))
+    k[0] *= np.linspace(0, 30, n)[:, None, None]      # ever larger scores
+    v[0] *= np.exp2(rng.integers(-30, 30, (n, 1, 1)))
+    k[1], q[1] = k[1] * 2.0 ** 100, q[1] * 2.0 ** -100
+    v[1, :, 0] *= 2.0 ** np.linspace(-70, 70, n)[:, None]
+    v[2, n // 2:] *= 2.0 ** 90
+    k, v, q = (x.astype(np.float32) for x in (k, v, q))
+    held = Held(batch, n, kvh, hd)
+    cache = pkg.hip.Q8Cache(backend, batch, n, kvh, hd)
+    _write(pkg, backend, cache, k, v, [0] * batch, None)
+    held.write(k, v, [0] * batch, [n] * batch)
+    prefix, pheld = _filled(pkg, backend, rng, 1, ahead, kvh, hd)
+    pos = [n - rows, n - rows - 60, n - rows - 1]
+    for pre, ph, some in ((None, None, 0), (prefix, pheld, ahead)):
+        got, lse = _attend(pkg, backend, q, cache, pos, None, 0.2, pre, some)
+        want, wl, tol, lt = attention(q, held, pos, [rows] * batch, 0.2, ph, some)
+        _close(got, want, tol)
+        _close(lse, wl, lt)
+
+
+@gpu
+@pytest.mark.parametrize("rows,batch,kvh,hd,most", [(1, 3, 2, 64, 2400), (6, 20, 3, 128, 1500),
+                                                    (30, 2, 2, 64, 2400)])
+def test_rows_that_are_not_there(backend, pkg, rows, batch, kvh, hd, most):
+    # What q holds in rows behind counts reaches no other row: NaN, infinities
+    # and large numbers there change no bit, with and without a prefix.
+    rng = np.random.default_rng(rows)
+    cache, _ = _filled(pkg, backend, rng, batch, most, kvh, hd)
+    prefix, _ = _filled(pkg, backend, rng, 1, 500, kvh, hd)
+    q = rng.standard_normal((batch, rows, kvh, hd)).astype(np.float32)
+    counts = [(i * 7) % (rows + 1) for i in range(batch)]
+    behind = np.arange(rows) >= np.array(counts)[:, None]
+    pos = [most - rows - 31 * i for i in range(batch)]
+    for pre, ahead in ((None, 0), (prefix, 500)):
+        q[behind] = 0
+        want = _attend(pkg, backend, q, cache, pos, counts, 0.125, pre, ahead)
+        for fill in (np.nan, np.inf, -3e38, 1e4):
+            q[behind] = fill
+            got = _attend(pkg, backend, q, cache, pos, counts, 0.125, pre, ahead)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        assert (want[0][behind] == 0).all() and np.isneginf(want[1][behind]).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 4])
+def test_attention_over_a_large_cache(backend, pkg, rows):
+    # Codes of more than the caches hold, read past them (134 MB): every
+    # sequence the same rows, so that one tells of all.
+    rng = np.random.default_rng(rows)
+    batch, kvh, hd, most = 64, 4, 128, 2048
+    k, v = (_rows(rng, 1, most, kvh, hd, 1) for _ in range(2))
+    held = Held(1, most, kvh, hd)
+    held.write(k, v, [0], [most])
+    cache = pkg.hip.Q8Cache(backend, batch, most, kvh, hd)
+    for at in range(0, most, 256):
+        part = [np.repeat(x[:, at:at + 256], batch, 0) for x in (k, v)]
+        _write(pkg, backend, cache, *part, [at] * batch, None)
+    q = np.repeat(rng.standard_normal((1, rows, 2 * kvh, hd)), batch, 0).astype(np.float32)
+    got, lse = _attend(pkg, backend, q, cache, [most - rows] * batch, None, 0.1)
+    want, wl, tol, lt = attention(q[:1], held, [most - rows], [rows], 0.1)
+    _close(got[:1], want, tol)
+    _close(lse[:1], wl, lt)
+    assert (got == got[:1]).all() and (lse == lse[:1]).all()
+
+
+@gpu
 @pytest.mark.parametrize("rows", [1, 12])
 def test_attention_and_nan(backend, pkg, rows):
     # A NaN row inside the attended ones and a NaN or infinite q make their
@@ -542,6 +616,9 @@ def test_rows_refusals(pkg):
         assert call(good, stride=127) == bad
         assert call(good, pos=None) == bad
         assert call(_cache_c(h, slots=1 << 20), batch=1 << 20, rows=1 << 20) == bad
+        # A grid of 2^24 blocks or more.
+        assert call(_cache_c(h, slots=1 << 24), batch=1 << 24, rows=1) == bad
+        assert call(_cache_c(h, slots=1 << 24), batch=1 << 24, rows=4) == bad
         assert call(good, batch=0) == 0 and call(good, rows=0) == 0
     assert write(good, k=None) == bad and write(good, v=None) == bad
     assert write(good, backend=None) == bad
@@ -564,7 +641,7 @@ def test_attention_refusals(pkg):
     for prefix in (None, _cache_c(h, slots=1, max_rows=1000)):
         for kw in ({"batch": 5}, {"heads": 3}, {"heads": 0}, {"q_stride": 255},
                    {"out_stride": 255}, {"scale": float("nan")}, {"scale": float("inf")},
-                   {"q": None}, {"out": None}, {"pos": None}, {"rows": 1 << 22},
+                   {"q": None}, {"out": None}, {"pos": None}, {"rows": 1 << 22}, {"rows": 1 << 20},
                    {"cache": _cache_c(h, data=None)}, {"cache": _cache_c(h, data=24)},
                    {"cache": _cache_c(h, kv_heads=3)}, {"cache": _cache_c(h, head_dim=200)}):
             assert call(prefix=prefix, **kw) == bad, kw

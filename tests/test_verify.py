@@ -282,7 +282,8 @@ def test_refusals(pkg):
                {"n": (1 << 20) + 1}, {"rows": 1025}, {"batch": (1 << 20) + 1},
                {"temperature": float("nan")}, {"uniforms": None}, {"out": None}, {"kept": None},
                {"ws": None}, {"ws": C.c_void_p((1 << 21) + 8)}, {"size": need - 1},
-               {"batch": 1 << 20, "rows": 1024, "n": 1 << 20}):
+               {"batch": 1 << 20, "rows": 1024, "n": 1 << 20},
+               {"batch": 1 << 13, "rows": 1024, "n": 100}):
         assert call(**kw) == bad, kw
     assert call(batch=0) == 0
     with pytest.raises(h.InvalidArgument):
