@@ -329,8 +329,17 @@ struct Job {
     G = pl.G;
     group = 0;
     if (groups > 1) {
-      group = id % groups;
-      id /= groups;
+      // Blocks go to the eight XCDs in turn: those of the same keys to one, for its L2.
+      const uint32_t even = gridDim.x / groups / 8 * 8;
+      if (id < even * groups) {
+        const uint32_t k = id / 8;
+        group = k % groups;
+        id = k / groups * 8 + id % 8;
+      } else {
+        id -= even * groups;
+        group = id % groups;
+        id = even + id / groups;
+      }
     }
     kvh = id % a.c.kv_heads;
     id /= a.c.kv_heads;
@@ -970,7 +979,7 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
   }
 }
 
-// The same for jobs of 32 RW rows: the block's waves convert each stage of 64
+// The same for jobs of 32 RW rows (64 or 128): the block's waves convert each stage of 64
 // keys to fp16 once, into LDS in the order of the MFMAs' operands, and every wave
 // takes its 32 rows (wave % RW) over one of the stage's two 32-key tiles (wave / RW) from there;
 // the tiles' halves are joined at the end.  The next stage's codes are on
@@ -1362,46 +1371,58 @@ hipError_t launch_cache_read_q8(const Q8Cache& c, float* k, float* v, uint32_t b
 
 namespace {
 
-// Rows of a job: 8 in packed columns, 16, or 32, 64 and 128 by way of LDS.
-uint32_t rows_per_job(uint64_t rows) {
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-}
-
 constexpr uint64_t kCus = 256;
 
-// Blocks' waves and the splits of `tiles` 32-key tiles for `jobs` jobs of rt
-// rows, from a model of the time in us.  Direct jobs: a block takes 4 us and
-// each of a wave's tiles 0.85 us alone, 2.75 with the CUs full (8 waves of 128
-// columns, 12 of 64, per CU); jobs in LDS: 8 us and 2.1 us a stage of two
-// tiles.  Several splits cost a join, and their rows written and read.
+// How `jobs` (kv heads of sequences, or of the prefix) of `rows` query rows
+// each and `tiles` 32-key tiles are dealt: rows of a block (8 in packed
+// columns, 16, or 64 and 128 by way of LDS), its waves, and splits of the
+// keys, from a model of the time in us.  Direct blocks: 4.5 or 5 us (2 more where
+// CUs get a second one), and each of a wave's tiles 0.85 alone; with the CUs full (8
+// waves of 128 columns, 12 of 64) 1.65 or 2, or 2.75 where the codes come from
+// memory and no other group reads them.  Blocks in LDS: 8 of their waves on a
+// CU, 7 or 8.5 us and 1.4 to 2.8 or 2.1 a stage of 64 keys.  Splits cost a join, and
+// their rows written and read.  Over 72 shapes drawn from 1 to 256 rows and 64 to
+// 30000 keys the choice's time is 1.2% above the fastest kind's of rows per block, 20% at
+// the worst; taking the largest block that the rows fill was up to 2 times it
+// (16 x 20 rows of 12 heads over 2, 400 keys: 17.8 us, here 8.5).
 struct Deal {
-  uint32_t waves, splits;
+  uint32_t rt, groups, waves, splits;
 };
-Deal deal(uint64_t jobs, uint64_t tiles, uint32_t rt, uint32_t row, uint64_t ids, bool joined) {
+Deal deal(uint64_t jobs, uint64_t rows, uint64_t tiles, uint32_t row, uint64_t ids, bool joined) {
   static const uint32_t kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 21, 25, 32, 42, 51, 64};
-  Deal best{rt == 32 ? 2u : rt <= 64 ? 4u : 8u, 1};
-  double least = 1e30;
-  for (uint32_t w = rt <= 16 ? 2 : best.waves; w <= (rt <= 16 ? 4 : best.waves); w += 2)
-    for (uint32_t s : kSplits) {
-      if (s > kAttnMaxSplits || jobs * s * w > kMaxBlocks * 4 ||
-          (s > 1 && tiles / s < (rt <= 16 ? 2 * w : 4))) break;
-      const double cap = (double)kCus * (rt > 16 ? (rt == 32 && row == 128 ? 4 : 8)
-                                                 : row == 64 ? 12 : 8);
-      const double full = (double)(jobs * s * w) / cap;
-      const double rounds = full <= 1 ? 1 : full <= 4 ? (double)(uint64_t)(full + 0.999) : full;
-      const double at_once = full < 1 ? full : 1;
-      const double per = (double)div_up(tiles, (uint64_t)s * w);
-      double t = rt <= 16 ? rounds * (4 + per * (0.85 + 1.9 * at_once))
-                          : rounds * (8 + (double)div_up(tiles, 2 * (uint64_t)s) * 2.1);
-      if (s > 1 || joined) t += (double)ids * s * row * 8 / 4e6;
-      if (s > 1 && !joined) t += 4;
-      if (w == 2 && rt <= 16) t *= 1.05;  // four waves even out a block's tail
-      if (t < least) {
-        least = t;
-        best.splits = s;
-        best.waves = w;
+  Deal best{};
+  double least = 1e300;
+  for (uint32_t rt : {8u, 16u, 64u, 128u}) {
+    if (rt > 8 && rt / 2 >= rows && rt != 64) break;
+    if (rt == 64 && rows <= 16) break;
+    const bool direct = rt <= 16;
+    const uint64_t groups = div_up(rows, rt), blocks = jobs * groups;
+    const double cap = (double)kCus * (direct && row == 64 ? 12 : 8);
+    const double shared = std::max(rt == 8 ? 0.8 : 1.15, 1.9 / (double)groups);
+    const uint32_t most = direct ? 4 : rt / 16;
+    for (uint32_t w = rt == 8 ? 2 : most; w <= most; w += 2)  // (2 waves of 16 rows spill)
+      for (uint32_t s : kSplits) {
+        if (s > 1 && (s > kAttnMaxSplits || blocks * s * w > kMaxBlocks * 4 ||
+                      tiles / s < (direct ? 2 * w : 4)))
+          break;
+        const double full = (double)(blocks * s * w) / cap;
+        const double rounds = full <= 1 ? 1 : full <= 4 ? (double)(uint64_t)(full + 0.999) : full;
+        const double at_once = full < 1 ? full : 1;
+        const double second = std::min(std::max((double)(blocks * s * w) / (4 * kCus) - 1, 0.0), 1.0);
+        double t = direct ? (rt == 8 ? 4.5 : 5) + 2 * second + (double)div_up(tiles, (uint64_t)s * w) *
+                                                      (0.85 + shared * at_once)
+                   : rt == 64 ? 7 + (double)div_up(tiles, 2 * (uint64_t)s) * (1.4 + 1.4 * at_once)
+                              : 8.5 + (double)div_up(tiles, 2 * (uint64_t)s) * 2.1;
+        t *= rounds;
+        if (s > 1 || joined) t += (double)ids * s * row * 8 / 6e6;
+        if (s > 1 && !joined) t += 4;
+        if (w == 2) t *= 1.05;  // four waves even out a block's tail
+        if (t < least) {
+          least = t;
+          best = {rt, (uint32_t)groups, w, s};
+        }
       }
-    }
+  }
   return best;
 }
 
@@ -1411,10 +1432,10 @@ AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   p.G = (uint32_t)G;
   const uint64_t own = a.rows * G, all = own * a.batch;
   const uint64_t ids = (uint64_t)a.batch * a.rows * a.heads;
-  p.own_rt = rows_per_job(own);
-  p.own_groups = (uint32_t)div_up(own, p.own_rt);
-  const Deal d = deal((uint64_t)a.batch * a.c.kv_heads * p.own_groups, div_up(a.max_len, 32),
-                      p.own_rt, a.c.row, ids, false);
+  const Deal d = deal((uint64_t)a.batch * a.c.kv_heads, own, div_up(a.max_len, 32), a.c.row, ids,
+                      false);
+  p.own_rt = d.rt;
+  p.own_groups = d.groups;
   p.own_splits = d.splits;
   p.own_waves = d.waves;
   // Caches that the 256 MB behind the L2s will not hold until they are read
@@ -1422,10 +1443,9 @@ AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   // 256 rows (68 MB) 17.2 and 15.9, 512 27.9 and 30.2, 2048 88.3 and 96.7.
   p.stream = (uint64_t)a.batch * a.c.kv_heads * a.max_len * 2 * a.c.row > (96ull << 20);
   if (prefix) {  // its parts are joined with the own rows' in any case
-    p.prefix_rt = rows_per_job(all);
-    p.prefix_groups = (uint32_t)div_up(all, p.prefix_rt);
-    const Deal e = deal((uint64_t)a.c.kv_heads * p.prefix_groups, div_up(a.pre.max_rows, 32),
-                        p.prefix_rt, a.c.row, ids, true);
+    const Deal e = deal(a.c.kv_heads, all, div_up(a.pre.max_rows, 32), a.c.row, ids, true);
+    p.prefix_rt = e.rt;
+    p.prefix_groups = e.groups;
     p.prefix_splits = e.splits;
     p.prefix_waves = e.waves;
   }
@@ -1443,14 +1463,14 @@ void launch_parts(const AttnQ8Args& a, const AttnQ8Plan& p, hipStream_t s) {
   const uint32_t waves = SHARED ? p.prefix_waves : p.own_waves;
   auto direct = [&](auto pack) {
     constexpr bool PACK = decltype(pack)::value;
+    constexpr int FEW = PACK ? 2 : 4;
     if constexpr (!SHARED)
       if (p.stream)
-        return waves == 2 ? k_attn_q8<ROW, PACK, 2, false, true> : k_attn_q8<ROW, PACK, 4, false, true>;
-    return waves == 2 ? k_attn_q8<ROW, PACK, 2, SHARED, false> : k_attn_q8<ROW, PACK, 4, SHARED, false>;
+        return waves == 2 ? k_attn_q8<ROW, PACK, FEW, false, true> : k_attn_q8<ROW, PACK, 4, false, true>;
+    return waves == 2 ? k_attn_q8<ROW, PACK, FEW, SHARED, false> : k_attn_q8<ROW, PACK, 4, SHARED, false>;
   };
   auto* f = rt == 8    ? direct(std::true_type{})
             : rt == 16 ? direct(std::false_type{})
-            : rt == 32 ? k_attn_q8_rows<ROW, 1, SHARED>
             : rt == 64 ? k_attn_q8_rows<ROW, 2, SHARED>
                        : k_attn_q8_rows<ROW, 4, SHARED>;
   const uint32_t threads = waves * 64;

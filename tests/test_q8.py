@@ -51,8 +51,9 @@ class Held:
                         which[b, :, int(pos[b]) + t] = q[b, t]
 
 
-def attention(q, held, pos, counts, scale, prefix=None, prefix_len=0):
-    """(out, lse, out bound, lse bound) of q float32 [batch, rows, heads, hd]."""
+def attention(q, held, pos, counts, scale, prefix=None, prefix_len=0, pick=None):
+    """(out, lse, out bound, lse bound) of q float32 [batch, rows, heads, hd];
+    pick: of these (b, t, h) only."""
     batch, rows, heads, hd = q.shape
     group = heads // held.shape[2]
     out = np.zeros(q.shape)
@@ -62,6 +63,8 @@ def attention(q, held, pos, counts, scale, prefix=None, prefix_len=0):
         for t in range(min(int(counts[b]), rows)):
             n = min(int(pos[b]) + t + 1, held.shape[1])
             for h in range(heads):
+                if pick is not None and (b, t, h) not in pick:
+                    continue
                 k, v = held.k[b, h // group, :n], held.v[b, h // group, :n]
                 if prefix is not None:
                     m = min(prefix_len, prefix.shape[1])
@@ -411,6 +414,41 @@ def test_attention_of_uneven_rows(backend, pkg, rows, heads, kvh, hd):
         want, wl, tol, lt = attention(q, held, pos, [rows] * batch, 0.2, ph, some)
         _close(got, want, tol)
         _close(lse, wl, lt)
+
+
+@gpu
+@pytest.mark.parametrize("batch,rows,heads,kvh,hd,length,ahead", [
+    (4, 16, 32, 4, 100, 4000, 0), (2, 128, 8, 8, 50, 8000, 0), (16, 33, 8, 8, 80, 3500, 0),
+    (32, 64, 16, 16, 128, 500, 0), (32, 128, 8, 8, 64, 700, 0), (64, 33, 16, 16, 64, 400, 0),
+    (40, 1, 16, 16, 128, 3, 20000), (64, 2, 16, 16, 128, 3, 8200), (64, 4, 16, 4, 64, 40, 8200),
+    (20, 40, 16, 16, 128, 200, 4000), (20, 24, 16, 4, 64, 100, 4000),
+    (60, 1, 32, 32, 64, 2, 16000)])
+def test_attention_of_many_rows(backend, pkg, batch, rows, heads, kvh, hd, length, ahead):
+    # Enough rows and keys for blocks of 64 and 128 rows, with one split and
+    # with several; a sample of the rows against 64 bits.
+    rng = np.random.default_rng(batch + rows + length)
+    lens = [max(1, length - 13 * i) for i in range(batch)]
+    counts = [min(n, max(0, rows - 5 * (i % 4)) if rows > 4 else rows - i % (rows + 1))
+              for i, n in enumerate(lens)]
+    pos = [n - c for n, c in zip(lens, counts)]
+    cache, held = _filled(pkg, backend, rng, batch, length, kvh, hd)
+    _poison(pkg, backend, cache, lens)
+    prefix = pheld = None
+    if ahead:
+        prefix, pheld = _filled(pkg, backend, rng, 1, ahead + 30, kvh, hd)
+        _poison(pkg, backend, prefix, [ahead])
+    q = rng.standard_normal((batch, rows, heads, hd)).astype(np.float32)
+    got, lse = _attend(pkg, backend, q, cache, pos, counts, hd ** -0.5, prefix, ahead)
+    pick = {(int(rng.integers(batch)), int(rng.integers(rows)), int(rng.integers(heads)))
+            for _ in range(150)}
+    pick |= {(b, max(0, counts[b] - 1), heads - 1) for b in range(batch)}
+    want, wl, tol, lt = attention(q, held, pos, counts, hd ** -0.5, pheld, ahead, pick)
+    at = tuple(np.array(sorted(pick)).T)
+    _close(got[at], want[at], tol[at])
+    _close(lse[at], wl[at], lt[at])
+    behind = np.arange(rows) >= np.array(counts)[:, None]
+    assert (got[behind] == 0).all() and np.isneginf(lse[behind]).all()
+    assert np.isfinite(got).all() and np.isfinite(lse[~behind]).all()
 
 
 @gpu
