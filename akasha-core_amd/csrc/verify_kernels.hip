@@ -131,6 +131,7 @@ __device__ Step walk(double w, double base, double point, StepShared& sh) {
   return at;
 }
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // 2^(n + f) from m = 1.5 2^52 + n and |f| <= 1/2: the polynomial that agrees
 // with 2^f in the ten Chebyshev points of [-1/2, 1/2] (within 4e-14 of it, and
 // 1 at 0), n put into the exponent field as an integer: so every
@@ -146,9 +147,10 @@ __device__ __forceinline__ double power2(double m, double f) {
   p = fma(p, f, 0x1.ebfbdff8149f2p-3);
   p = fma(p, f, 0x1.62e42fefa39f7p-1);
   p = fma(p, f, 1.0);
-  const uint64_t u = __builtin_bit_cast(uint64_t, p);
-  const uint32_t hi = (uint32_t)(u >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, m) << 20);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
+  // (One instruction: in C the halves become a 64-bit sum of five.)
+  u32x2 u = __builtin_bit_cast(u32x2, p);
+  asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(u.y) : "v"(__builtin_bit_cast(u32x2, m).x));
+  return __builtin_bit_cast(double, u);
 }
 // Weight 2^(c (l - max)) of a logit next to its row's (or part's) maximum; none
 // for a NaN, and for an infinity next to an infinite maximum.  (Weights below
@@ -192,10 +194,11 @@ __device__ __forceinline__ void load_part(const float* row, uint32_t n, int part
 }
 
 // Rows of target first, then of draft.  32 sequences of 0 to 7 drafts over
-// 50257 ids (43 to 51 MB of live rows) take 16 to 17 us, 3 TB/s: the f64
-// arithmetic, 16 operations an id, is as long as the reads.  (With the first
-// maximum's index kept for every call and compares in place of the clamped exponent
-// it was 40 instructions an id and 22 us.)
+// 50257 ids, 256 rows live (51 MB), take 16 us, 3.1 TB/s, where a sum over 1 GB
+// reads at 4.1: the f64 arithmetic, 20 instructions an id, is half of that
+// long and the reads' start and end are seen.  (40 instructions, with the first
+// maximum's index kept in every call, compares and 64-bit exponent sums: 22
+// us; parts of 2048 ids 20 us; a sum next to each wave's own maximum the same.)
 __global__ __launch_bounds__(256) void k_verify_stats(VerifyArgs a, PartStat* stats, int* done,
                                                       int parts) {
   const uint32_t row = blockIdx.x / parts;
