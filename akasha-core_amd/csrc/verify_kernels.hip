@@ -19,7 +19,10 @@ namespace akh {
 namespace {
 
 constexpr int kPart = 4096;          // ids of a row that one block takes
-constexpr int kPer = kPart / 256;    // of them a thread's; consecutive ones are a chunk
+constexpr int kPer = kPart / 256;    // of them a thread's, for the statistics
+constexpr int kPick = 256;           // threads of a block for the last token
+constexpr int kChunk = kPart / kPick;  // ids of one of them, in a row
+constexpr int kWaves = kPick / 64;
 constexpr int kPreload = 16;         // parts whose chunk sums are fetched before one is chosen
 
 struct PartStat {
@@ -48,7 +51,7 @@ __device__ __forceinline__ double dpp_f64(double x) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 // Sum over aligned groups of 16 lanes (the partners of group_sum), over the
-// wave, over the block of 256; every lane gets it.
+// wave, over the block; every lane gets it.
 __device__ __forceinline__ double sum16_f64(double v) {
   v += dpp_f64<0xB1>(v);
   v += dpp_f64<0x4E>(v);
@@ -79,12 +82,16 @@ __device__ __forceinline__ double xor_sum_f64(double x) {
 __device__ __forceinline__ double wave_sum_f64(double v) {
   return xor_sum_f64<32>(xor_sum_f64<16>(sum16_f64(v)));
 }
-__device__ __forceinline__ double block_sum_f64(double v, double* red4) {
+template <int WAVES>
+__device__ __forceinline__ double block_sum_f64(double v, double* red) {
   v = wave_sum_f64(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red4[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  return ((red4[0] + red4[1]) + red4[2]) + red4[3];
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) v += red[i];
+  return v;
 }
 // Sum over the wave's lanes up to and with this one.
 __device__ __forceinline__ double wave_scan_f64(double v, int lane) {
@@ -95,7 +102,7 @@ __device__ __forceinline__ double wave_scan_f64(double v, int lane) {
   }
   return v;
 }
-// Where a walk over 256 threads' weights passes `point`, starting at `base`:
+// Where a walk over the block's weights passes `point`, starting at `base`:
 // the thread, and what lies before it.  Rounding may leave none past the
 // point: the last one with weight then.
 struct Step {
@@ -103,8 +110,8 @@ struct Step {
   double before;
 };
 struct StepShared {
-  double tot[4];
-  Step hit[4], last[4];  // of each wave; at < 0: none
+  double tot[kWaves];
+  Step hit[kWaves], last[kWaves];  // of each wave; at < 0: none
 };
 __device__ Step walk(double w, double base, double point, StepShared& sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -123,10 +130,10 @@ __device__ Step walk(double w, double base, double point, StepShared& sh) {
   __syncthreads();
   Step at = {0, base};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kWaves; ++i)
     if (sh.last[i].at >= 0) at = sh.last[i];
 #pragma unroll
-  for (int i = 3; i >= 0; --i)
+  for (int i = kWaves - 1; i >= 0; --i)
     if (sh.hit[i].at >= 0) at = sh.hit[i];
   return at;
 }
@@ -236,7 +243,7 @@ __global__ __launch_bounds__(256) void k_verify_stats(VerifyArgs a, PartStat* st
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) sum += weight_in_sum(x[i], best, c2, least);
-  sum = block_sum_f64(sum, red_d);
+  sum = block_sum_f64<4>(sum, red_d);
   if (threadIdx.x == 0)
     stats[blockIdx.x] = {fabsf(best) < INFINITY ? sum : 0.0, best, 0xFFFFFFFFu};
 }
@@ -297,19 +304,38 @@ __device__ __forceinline__ void agent_store(double* p, double x) {
   __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Slot of an id's logit in a part's LDS copy: four words apart every sixteen,
-// so that threads reading sixteen in a row keep off each other's banks.
-__device__ __forceinline__ int slot(int i) { return i + (i >> 4) * 4; }
+// A thread's kChunk ids in a row of a part; NaN past the row's end.
+__device__ __forceinline__ void load_chunk(const float* row, uint32_t n, int part, float* x) {
+  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+  const uint32_t here = min(n - (uint32_t)part * kPart, (uint32_t)kPart);
+  const float* p = row + (size_t)part * kPart;
+  const uint32_t at = threadIdx.x * kChunk;
+  if (here == kPart) {
+#pragma unroll
+    for (int i = 0; i < kChunk; i += 4) {
+      const f4 v = *reinterpret_cast<const f4*>(p + at + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[i + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) x[i] = p[min(at + i, here - 1)];
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (at + i >= here) x[i] = NAN;
+  }
+}
 
-// A chain of loads and short scans, each waiting for the one before it: 11 us
-// for one sequence, 15 us for 32 (two rows of 50257 ids each, 13 MB, and the
-// rest of the chip idle).  As a launch of its own after one that sums the chunks it was
-// 8 us on top of 16; the hand-off to the last block costs 1.4.
+// A chain of loads and short scans, each waiting for the one before it: 10 us
+// for one sequence, 14 us for 32 (two rows of 50257 ids each, 13 MB). As a
+// launch of its own after one that sums the chunks it was 8 us on top of 16; the
+// hand-off to the last block costs 1.4.  Blocks of 512 or 1024 threads with
+// chunks of 8 or 4 ids: 11.5 and 16 us; the parts' logits by way of LDS 10.9.
 // A block per sequence and part (one part when greedy).  Every block joins
 // the sequence's rows, 16 at a time with 16 lanes each, up to the first refused draft.
 // The sums are written through to device scope and counted there; the count
 // starts at zero by k_verify_stats.
-__global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartStat* stats,
+__global__ __launch_bounds__(kPick) void k_verify_pick(VerifyArgs a, const PartStat* stats,
                                                      double* sums, double* totals, int* done,
                                                      int parts) {
   const bool greedy = !(a.temperature > 0.f);
@@ -368,7 +394,7 @@ __global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartSta
       }
     }
     __syncthreads();
-    if (!decided && refused < t0 + 16) {
+    if (!decided && refused < t0 + kPick / 16) {
       if (t == refused && lane16 == 0) {
         dec.p = p;
         dec.q = q;
@@ -379,12 +405,12 @@ __global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartSta
       decided = true;
       if (part != 0) break;
     }
-    t0 += 16;
+    t0 += kPick / 16;
   } while (t0 <= c);
   __syncthreads();
   const Decision d = dec;
   if (part == 0) {
-    for (uint32_t t = threadIdx.x; t <= a.rows; t += 256) {
+    for (uint32_t t = threadIdx.x; t <= a.rows; t += kPick) {
       if (t != d.row)
         a.out_tokens[trow + t] = t < d.row ? a.tokens[(size_t)b * a.rows + t] : 0xFFFFFFFFu;
       if (t >= c && t < a.rows && a.chance) a.chance[(size_t)b * a.rows + t] = 0.f;
@@ -406,38 +432,21 @@ __global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartSta
   w.c = c2;
   w.inv_p = d.p.sum > 0.0 ? 1.0 / d.p.sum : 0.0;
   w.inv_q = d.q.sum > 0.0 ? 1.0 / d.q.sum : 0.0;
-  // The part's logits, by way of LDS into threads of sixteen consecutive ids.
-  constexpr int kSlots = kPart + kPart / 4;
-  __shared__ __attribute__((aligned(16))) float xs[2][kSlots];
-  __shared__ double red[4];
+  __shared__ double red[kWaves];
   {
-    float x[kPer], y[kPer];
-    load_part(w.p, a.n, part, x);
-    if (w.q) load_part(w.q, a.n, part, y);
+    float x[kChunk], y[kChunk] = {};
+    load_chunk(w.p, a.n, part, x);
+    if (w.q) load_chunk(w.q, a.n, part, y);
+    if (w.less_q && !w.q) {
+      const uint32_t one = w.token - (part * kPart + threadIdx.x * kChunk);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = i * 256 + threadIdx.x;
-      xs[0][slot(id)] = x[i];
-      if (w.q) xs[1][slot(id)] = y[i];
+      for (int i = 0; i < kChunk; ++i) y[i] = one == (uint32_t)i ? 1.f : 0.f;
     }
-    __syncthreads();
     double own = 0.0;
-    const uint32_t id0 = part * kPart + threadIdx.x * kPer;
 #pragma unroll
-    for (int i = 0; i < kPer; i += 4) {
-      const float4 lp = *reinterpret_cast<const float4*>(&xs[0][slot(threadIdx.x * kPer) + i]);
-      float4 lq = w.q ? *reinterpret_cast<const float4*>(&xs[1][slot(threadIdx.x * kPer) + i])
-                      : make_float4(0.f, 0.f, 0.f, 0.f);
-      if (w.less_q && !w.q) {
-        lq.x = w.token == id0 + i ? 1.f : 0.f;
-        lq.y = w.token == id0 + i + 1 ? 1.f : 0.f;
-        lq.z = w.token == id0 + i + 2 ? 1.f : 0.f;
-        lq.w = w.token == id0 + i + 3 ? 1.f : 0.f;
-      }
-      own += (w.of(lp.x, lq.x) + w.of(lp.y, lq.y)) + (w.of(lp.z, lq.z) + w.of(lp.w, lq.w));
-    }
-    agent_store(sums + ((size_t)b * parts + part) * 256 + threadIdx.x, own);
-    const double total = block_sum_f64(own, red);
+    for (int i = 0; i < kChunk; ++i) own += w.of(x[i], y[i]);
+    agent_store(sums + ((size_t)b * parts + part) * kPick + threadIdx.x, own);
+    const double total = block_sum_f64<kWaves>(own, red);
     if (threadIdx.x == 0) agent_store(totals + (size_t)b * parts + part, total);
   }
   __builtin_amdgcn_s_waitcnt(0);
@@ -449,34 +458,34 @@ __global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartSta
   __syncthreads();
   if (!last_block) return;
 
-  double* s = sums + (size_t)b * parts * 256 + threadIdx.x;
+  double* s = sums + (size_t)b * parts * kPick + threadIdx.x;
   uint32_t* out = a.out_tokens + trow + d.row;
   double v[kPreload];
 #pragma unroll
-  for (int i = 0; i < kPreload; ++i) v[i] = i < parts ? agent_load(s + (size_t)i * 256) : 0.0;
+  for (int i = 0; i < kPreload; ++i) v[i] = i < parts ? agent_load(s + (size_t)i * kPick) : 0.0;
   double mine = (int)threadIdx.x < parts ? agent_load(totals + (size_t)b * parts + threadIdx.x) : 0.0;
-  double total = block_sum_f64(mine, red);
+  double total = block_sum_f64<kWaves>(mine, red);
   bool fetched = parts <= kPreload;
   if (!(total > 0.0) && w.less_q) {
     // Nothing of p exceeds q: p itself, whose sums are made here.
     w.less_q = false;
     for (int i = 0; i < parts; ++i) {
       double own = 0.0;
-      for (int k = 0; k < kPer; ++k)
-        own += w.of_id((uint32_t)i * kPart + threadIdx.x * kPer + k, a.n);
-      agent_store(s + (size_t)i * 256, own);
-      const double sum = block_sum_f64(own, red);
+      for (int k = 0; k < kChunk; ++k)
+        own += w.of_id((uint32_t)i * kPart + threadIdx.x * kChunk + k, a.n);
+      agent_store(s + (size_t)i * kPick, own);
+      const double sum = block_sum_f64<kWaves>(own, red);
       if ((int)threadIdx.x == i) mine = sum;
     }
     __builtin_amdgcn_s_waitcnt(0);
-    total = block_sum_f64(mine, red);
+    total = block_sum_f64<kWaves>(mine, red);
     fetched = false;
   }
   if (!(total > 0.0)) {  // no weight at all: the row's first maximum
     __syncthreads();
     if (threadIdx.x == 0) refused = a.n;
     __syncthreads();
-    for (uint32_t id = threadIdx.x; id < a.n; id += 256)
+    for (uint32_t id = threadIdx.x; id < a.n; id += kPick)
       if (w.p[id] == w.pm) {
         atomicMin(&refused, id);
         break;
@@ -493,11 +502,11 @@ __global__ __launch_bounds__(256) void k_verify_pick(VerifyArgs a, const PartSta
 #pragma unroll
     for (int i = 0; i < kPreload; ++i) chunk = i == at.at ? v[i] : chunk;
   } else {
-    chunk = agent_load(s + (size_t)at.at * 256);
+    chunk = agent_load(s + (size_t)at.at * kPick);
   }
   const Step in = walk(chunk, at.before, point, sh);
-  const uint32_t id0 = (uint32_t)at.at * kPart + in.at * kPer;
-  const Step id = walk(threadIdx.x < kPer ? w.of_id(id0 + threadIdx.x, a.n) : 0.0, in.before,
+  const uint32_t id0 = (uint32_t)at.at * kPart + in.at * kChunk;
+  const Step id = walk(threadIdx.x < kChunk ? w.of_id(id0 + threadIdx.x, a.n) : 0.0, in.before,
                        point, sh);
   if (threadIdx.x == 0) *out = id0 + id.at;
 }
@@ -513,20 +522,20 @@ uint64_t verify_blocks(uint32_t batch, uint32_t rows, uint32_t n) {
 
 size_t verify_workspace_bytes(uint32_t batch, uint32_t rows, uint32_t n) {
   return verify_blocks(batch, rows, n) * sizeof(PartStat) +
-         (size_t)batch * (parts_of(n) * 257 * sizeof(double) + sizeof(int));
+         (size_t)batch * (parts_of(n) * (kPick + 1) * sizeof(double) + sizeof(int));
 }
 
 hipError_t launch_verify(const VerifyArgs& a, hipStream_t s) {
   const int parts = parts_of(a.n);
   PartStat* stats = static_cast<PartStat*>(a.ws);
   double* sums = reinterpret_cast<double*>(stats + verify_blocks(a.batch, a.rows, a.n));
-  double* totals = sums + (size_t)a.batch * parts * 256;
+  double* totals = sums + (size_t)a.batch * parts * kPick;
   int* done = reinterpret_cast<int*>(totals + (size_t)a.batch * parts);
   const uint64_t rows = a.draft ? stat_rows(a.batch, a.rows) : (uint64_t)a.batch * (a.rows + 1);
   hipLaunchKernelGGL(k_verify_stats, dim3((uint32_t)(rows * parts)), dim3(256), 0, s, a, stats,
                      done, parts);
   hipLaunchKernelGGL(k_verify_pick, dim3(a.temperature > 0.f ? a.batch * parts : a.batch),
-                     dim3(256), 0, s, a, stats, sums, totals, done, parts);
+                     dim3(kPick), 0, s, a, stats, sums, totals, done, parts);
   return hipGetLastError();
 }
 
