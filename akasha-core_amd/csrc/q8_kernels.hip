@@ -610,7 +610,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       float big = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
-      over |= big > 61440.f || add[n] > 0x1p110f;
+      over |= big > 61440.f || add[n] > 0x1p96f;
     }
   }
   if (__any(over)) {
@@ -636,7 +636,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       }
       st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
-      float m1 = fmaxf(st.top_w[n] - (float)eb1 - (PACK ? 3.f : 6.f), st.top_x[n] - 100.f);
+      float m1 = fmaxf(st.top_w[n] - (float)eb1 - (PACK ? 3.f : 6.f), st.top_x[n] - 90.f);  // (2^30 sums stay in f32)
       if (m1 == -INFINITY) m1 = 0.f;  // no key yet
       if (!st.fresh) {
         st.l[n] *= __builtin_amdgcn_exp2f(st.mt[n] - m1);

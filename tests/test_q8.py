@@ -617,6 +617,38 @@ def test_same_call_twice_is_the_same(backend, pkg):
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
 
 
+@gpu
+def test_backends_side_by_side(pkg):
+    # Two backends' calls (streams and workspaces of their own) under way at
+    # once over one cache's rows give what each gives alone.
+    h = pkg.hip
+    a, b = h.Backend(0), h.Backend(0)
+    try:
+        rng = np.random.default_rng(21)
+        batch, heads, kvh, hd, most = 8, 8, 4, 128, 3000
+        cache, _ = _filled(pkg, a, rng, batch, most, kvh, hd)
+        a.synchronize()
+        seen = h.Q8Cache(b, batch, most, kvh, hd, data=cache.data)
+        q = [rng.standard_normal((batch, rows, heads, hd)).astype(np.float32) for rows in (1, 6)]
+        alone = [_attend(pkg, a, x, cache, [most - 6] * batch, None, 0.1)[0] for x in q]
+        calls = []
+        for be, c, x in ((a, cache, q[0]), (b, seen, q[1])):
+            rows = x.shape[1]
+            shape = h.AttnQ8(batch, rows, heads, heads * hd, heads * hd, 0.1, 0)
+            size = h.attn_q8_workspace(shape, c)
+            calls.append((be, be.tensor(x), c, be.zeros(x.size), shape, _u32(be, [most - 6] * batch),
+                          be.zeros(size // 4 + 1), size))
+        a.synchronize(), b.synchronize()
+        for _ in range(20):
+            for be, dq, c, out, shape, pos, ws, size in calls:
+                be.attn_cached_q8(dq, c, out, None, shape, pos, None, ws, size)
+        for (be, _, _, out, *_), x, want in zip(calls, q, alone):
+            assert np.array_equal(out.download().reshape(x.shape), want)
+    finally:
+        b.close()
+        a.close()
+
+
 # ---- refusals ----------------------------------------------------------------
 
 
