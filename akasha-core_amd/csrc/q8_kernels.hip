@@ -204,9 +204,13 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
 //
 // The exponents: a key's K scale multiplies its scores, its V scale its
 // weights.  Weights are kept at 2^(x - mt) 2^(ve - eb) with mt (per row) and
-// eb (per wave) such that the largest lies at 2^6 (PACK: 2^3), whole powers of
+// eb (per wave) such that the largest lies at 2^0 (PACK: 2^-3), whole powers of
 // two; they may grow to 61440 before mt and eb move and the accumulators are rescaled
-// (exactly), so most tiles neither join maxima across lanes nor rescale.
+// (exactly), so most tiles neither join maxima across lanes nor rescale.  A
+// weight loses what is below 2^-25 (its lo's last bit), PACK's 2^-36.  With the
+// largest at 2^6 the levels of 32 rows moved so often that the barriers of
+// blocks in LDS waited for one wave or another: 69 us in place of 62 behind 8200
+// keys whose scales differ by 16, the errors against 64 bits the same to 8%.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -243,10 +247,12 @@ __device__ __forceinline__ uint32_t pair_f16(uint32_t a, uint32_t b) {
 // bits, lo the rest rounded to 11 (together within 2^-22, or 2^-25 below fp16's
 // normal range).
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
-  const h2 l = {(_Float16)fmaf((float)h[0], -1.f, a), (_Float16)fmaf((float)h[1], -1.f, b)};
-  hi = __builtin_bit_cast(uint32_t, h);
-  lo = __builtin_bit_cast(uint32_t, l);
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  // lo = x - hi in one instruction each (in C they become conversions and sums, three).
+  asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(a));
+  asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+      : "+v"(lo)
+      : "v"(hi), "v"(b));
 }
 
 __device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
@@ -614,7 +620,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     }
   }
   if (__any(over)) {
-    // New levels: the largest x + ve of a row at 2^6 or 2^3.  eb is 0 unless the
+    // New levels: the largest x + ve of a row at 2^0 or 2^-3.  eb is 0 unless the
     // values' scales are far from 1.
     asm volatile("");
     int high = -126;
@@ -636,7 +642,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       }
       st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
-      float m1 = fmaxf(st.top_w[n] - (float)eb1 - (PACK ? 3.f : 6.f), st.top_x[n] - 90.f);  // (2^30 sums stay in f32)
+      float m1 = fmaxf(st.top_w[n] - (float)eb1 - (PACK ? -3.f : 0.f), st.top_x[n] - 90.f);  // (2^30 sums stay in f32)
       if (m1 == -INFINITY) m1 = 0.f;  // no key yet
       if (!st.fresh) {
         st.l[n] *= __builtin_amdgcn_exp2f(st.mt[n] - m1);
@@ -996,13 +1002,13 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
 // their way while a stage is computed, and are converted into the other half
 // of the buffer.
 //
-// 256 rows over 8200 keys of 16 heads of 128 take 59 us, 580 TFLOP/s of fp16 products
-// (both terms of q and of the weights counted): about 10 us before and after the loop, then 2.7
-// us a stage.  Of a stage's 1000 cycles of MFMAs a wave and 1450 of vector
-// operations (363 a tile: exponents, 2^x, splitting the weights) the two waves of a SIMD overlap
-// little.  Stages of 128 keys, wave priorities (by half, or around the
-// products), and exponents fetched ahead measured within 2% of this; 64
-// keys' codes two stages ahead too.
+// 256 rows over 8200 keys of 16 heads of 128 take 52 us: about 10 before and after
+// the loop, then 1.9 us a stage (1040 TFLOP/s of fp16 products, both terms of q
+// and of the weights counted), more where levels move.  A stage is 1000
+// cycles of MFMAs a wave and 1350 of vector operations (exponents, 2^x, splitting the
+// weights, converting codes), two waves a SIMD.  Stages of 128 keys, codes two stages
+// ahead, wave priorities (by half, or around the products), exponents
+// fetched ahead, and levels moved by the weights' own exponents measured within 2%.
 template <int ROW, int RW, bool SHARED>
 __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, AttnQ8Plan pl) {
   constexpr int KS = ROW / 32, DT = ROW / 16, NT = 2, U = ROW / 64, W = 2 * RW;
