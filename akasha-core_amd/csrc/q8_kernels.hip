@@ -204,13 +204,14 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
 //
 // The exponents: a key's K scale multiplies its scores, its V scale its
 // weights.  Weights are kept at 2^(x - mt) 2^(ve - eb) with mt (per row) and
-// eb (per wave) such that the largest lies at 2^0 (PACK: 2^-3), whole powers of
-// two; they may grow to 61440 before mt and eb move and the accumulators are rescaled
-// (exactly), so most tiles neither join maxima across lanes nor rescale.  A
-// weight loses what is below 2^-25 (its lo's last bit), PACK's 2^-36.  With the
-// largest at 2^6 the levels of 32 rows moved so often that the barriers of
-// blocks in LDS waited for one wave or another: 69 us in place of 62 behind 8200
-// keys whose scales differ by 16, the errors against 64 bits the same to 8%.
+// eb (per wave) such that the largest lies at 2^-4, whole powers of two; they
+// may grow to 30720 (PACK: 61440) before mt and eb move and the accumulators are
+// rescaled (exactly), so most tiles neither join maxima across lanes nor
+// rescale.  lo is kept times 2^11 and meets V's codes times 2^-11 (PACK: its
+// column's results take the factor), so a weight loses what is below 2^-36 only, next to a
+// largest one of 2^-4.  With lo unscaled and levels at 2^6 the 32 rows of a
+// wave moved them so often that the barriers of blocks in LDS waited for one
+// wave or another: 69 us in place of 64 behind 8200 keys whose scales differ by 16.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -253,6 +254,19 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
       : "+v"(lo)
       : "v"(hi), "v"(b));
+}
+
+// The same with lo times 2^11 (a, b at most 30720), for weights: it keeps what lies below hi of
+// the smallest ones too.
+__device__ __forceinline__ void split2_up(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const float up = -2048.f;
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  asm("v_fma_mixlo_f16 %0, %1, %3, %2 op_sel_hi:[1,0,0]"
+      : "=v"(lo)
+      : "v"(hi), "v"(a * 2048.f), "s"(up));
+  asm("v_fma_mixhi_f16 %0, %1, %3, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+      : "+v"(lo)
+      : "v"(hi), "v"(b * 2048.f), "s"(up));
 }
 
 __device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
@@ -616,11 +630,11 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       float big = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
-      over |= big > 61440.f || add[n] > 0x1p96f;
+      over |= big > (PACK ? 61440.f : 30720.f) || add[n] > 0x1p96f;
     }
   }
   if (__any(over)) {
-    // New levels: the largest x + ve of a row at 2^0 or 2^-3.  eb is 0 unless the
+    // New levels: the largest x + ve of a row at 2^-4.  eb is 0 unless the
     // values' scales are far from 1.
     asm volatile("");
     int high = -126;
@@ -642,7 +656,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       }
       st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
-      float m1 = fmaxf(st.top_w[n] - (float)eb1 - (PACK ? -3.f : 0.f), st.top_x[n] - 90.f);  // (2^30 sums stay in f32)
+      float m1 = fmaxf(st.top_w[n] - (float)eb1 - -4.f, st.top_x[n] - 90.f);  // (2^30 sums stay in f32)
       if (m1 == -INFINITY) m1 = 0.f;  // no key yet
       if (!st.fresh) {
         st.l[n] *= __builtin_amdgcn_exp2f(st.mt[n] - m1);
@@ -684,7 +698,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split2(w[n][2 * i], w[n][2 * i + 1], h[i], o[i]);
+      for (int i = 0; i < 4; ++i) split2_up(w[n][2 * i], w[n][2 * i + 1], h[i], o[i]);
       pl[n] = f16x8_of(make_uint4(o[0], o[1], o[2], o[3]));
     }
     ph[n] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
@@ -701,10 +715,11 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       st.acc[n][j + 1] = mfma16(m1, ph[n], st.acc[n][j + 1]);
     }
     if constexpr (!PACK) {
+      const f16x8 s0 = m0 * (_Float16)0x1p-11f, s1 = m1 * (_Float16)0x1p-11f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        st.acc[n][j] = mfma16(m0, pl[n], st.acc[n][j]);
-        st.acc[n][j + 1] = mfma16(m1, pl[n], st.acc[n][j + 1]);
+        st.acc[n][j] = mfma16(s0, pl[n], st.acc[n][j]);
+        st.acc[n][j + 1] = mfma16(s1, pl[n], st.acc[n][j + 1]);
       }
     }
   }
@@ -1002,8 +1017,8 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
 // their way while a stage is computed, and are converted into the other half
 // of the buffer.
 //
-// 256 rows over 8200 keys of 16 heads of 128 take 52 us: about 10 before and after
-// the loop, then 1.9 us a stage (1040 TFLOP/s of fp16 products, both terms of q
+// 256 rows over 8200 keys of 16 heads of 128 take 53 us: about 10 before and after
+// the loop, then 2 us a stage (1000 TFLOP/s of fp16 products, both terms of q
 // and of the weights counted), more where levels move.  A stage is 1000
 // cycles of MFMAs a wave and 1350 of vector operations (exponents, 2^x, splitting the
 // weights, converting codes), two waves a SIMD.  Stages of 128 keys, codes two stages

@@ -618,6 +618,33 @@ def test_same_call_twice_is_the_same(backend, pkg):
 
 
 @gpu
+@pytest.mark.parametrize("batch,rows,heads,kvh,hd,n", [(1, 1, 2, 2, 64, 50000), (2, 12, 2, 2, 64, 20000),
+                                                      (1, 128, 16, 16, 128, 3000), (32, 64, 16, 16, 128, 500)])
+def test_one_key_next_to_many(backend, pkg, batch, rows, heads, kvh, hd, n):
+    # The first key weighs about as much as all others together, which weigh
+    # the same: whatever a small weight loses is lost n times over.
+    rng = np.random.default_rng(n)
+    u = rng.standard_normal(hd).astype(np.float32)
+    k = np.zeros((batch, n, kvh, hd), np.float32)
+    v = np.ones_like(k)
+    k[:, 0], v[:, 0] = u, 0
+    q = np.broadcast_to(u / (u @ u), (batch, rows, heads, hd)).astype(np.float32)
+    scale = float(np.float32(np.log(n) + 0.37))
+    cache = pkg.hip.Q8Cache(backend, batch, n, kvh, hd)
+    _write(pkg, backend, cache, k, v, [0] * batch, None)
+    got, lse = _attend(pkg, backend, q, cache, [n - rows] * batch, None, scale)
+    x0 = scale * (quantise(u[None])[0] @ q[0, 0, 0].astype(np.float64))
+    others = n - rows + np.arange(rows)
+    want = others / (others + np.exp(x0))
+    # The score is off by (hd + 8) 2^-23 of its products' magnitudes (their sum is near x0 < 12)
+    # and as an exponent of 2 by 2^-22; a weight by 2^-22; a wave adds n / 32 /
+    # 4 tiles in f32.
+    tol = 12 * (hd + 8) * 2.0 ** -23 + 12 * 2.0 ** -22 + 2.0 ** -21 + n / 128 * 2.0 ** -24
+    assert np.abs(got / want[:, None, None] - 1).max() <= tol
+    assert np.abs(lse - np.log(others + np.exp(x0))[:, None]).max() <= tol + 2.0 ** -20
+
+
+@gpu
 def test_backends_side_by_side(pkg):
     # Two backends' calls (streams and workspaces of their own) under way at
     # once over one cache's rows give what each gives alone.
