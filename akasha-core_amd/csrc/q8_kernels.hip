@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
 // The exponents: a key's K scale multiplies its scores, its V scale its
 // weights.  Weights are kept at 2^(x - mt) 2^(ve - eb) with mt (per row) and
 // eb (per wave) such that the largest lies at 2^-4, whole powers of two; they
-// may grow to 30720 (PACK: 61440) before mt and eb move and the accumulators are
+// may grow to 2^15 (PACK: 61440) before mt and eb move and the accumulators are
 // rescaled (exactly), so most tiles neither join maxima across lanes nor
 // rescale.  lo is kept times 2^11 and meets V's codes times 2^-11 (PACK: its
 // column's results take the factor), so a weight loses what is below 2^-36 only, next to a
@@ -256,7 +256,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
       : "v"(hi), "v"(b));
 }
 
-// The same with lo times 2^11 (a, b at most 30720), for weights: it keeps what lies below hi of
+// The same with lo times 2^11 (a, b at most 2^15), for weights: it keeps what lies below hi of
 // the smallest ones too.
 __device__ __forceinline__ void split2_up(float a, float b, uint32_t& hi, uint32_t& lo) {
   const float up = -2048.f;
@@ -630,7 +630,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
       float big = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) big = fmaxf(big, w[n][i]);
-      over |= big > (PACK ? 61440.f : 30720.f) || add[n] > 0x1p96f;
+      over |= big > (PACK ? 61440.f : 0x1p15f) || add[n] > 0x1p96f;
     }
   }
   if (__any(over)) {
