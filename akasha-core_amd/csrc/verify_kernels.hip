@@ -511,6 +511,7 @@ __global__ __launch_bounds__(kPick) void k_verify_pick(VerifyArgs a, const PartS
   if (threadIdx.x == 0) *out = id0 + id.at;
 }
 
+static_assert(kMaxSampleVocab / kPart <= kPick, "a thread a part of a row");
 int parts_of(uint32_t n) { return (int)((n + kPart - 1) / kPart); }
 uint64_t stat_rows(uint32_t batch, uint32_t rows) { return (uint64_t)batch * (2 * (uint64_t)rows + 1); }
 

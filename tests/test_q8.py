@@ -452,6 +452,32 @@ def test_attention_of_many_rows(backend, pkg, batch, rows, heads, kvh, hd, lengt
 
 
 @gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd,batch", [(700, 4, 2, 64, 2), (515, 16, 16, 128, 4),
+                                                     (1029, 32, 8, 112, 2)])
+def test_attention_of_a_whole_prompt(backend, pkg, rows, heads, kvh, hd, batch):
+    # Every row sees one key more than the row before it, from the first.
+    rng = np.random.default_rng(rows)
+    cache, held = _filled(pkg, backend, rng, batch, rows + 40, kvh, hd)
+    prefix, pheld = _filled(pkg, backend, rng, 1, 70, kvh, hd)
+    q = rng.standard_normal((batch, rows, heads, hd)).astype(np.float32)
+    pos = [0, 37, 5, 1][:batch]
+    counts = [rows, rows - 3, 0, 200][:batch]
+    _poison(pkg, backend, cache, [p + c for p, c in zip(pos, counts)])
+    pick = {(b, t, h) for b in range(batch) for t in (0, 1, 31, 32, 130, rows - 4, rows - 1)
+            for h in (0, heads - 1)}
+    pick |= {(int(rng.integers(batch)), int(rng.integers(rows)), int(rng.integers(heads)))
+             for _ in range(60)}
+    at = tuple(np.array(sorted(pick)).T)
+    behind = np.arange(rows) >= np.array(counts)[:, None]
+    for pre, ph, ahead in ((None, None, 0), (prefix, pheld, 70)):
+        got, lse = _attend(pkg, backend, q, cache, pos, counts, hd ** -0.5, pre, ahead)
+        want, wl, tol, lt = attention(q, held, pos, counts, hd ** -0.5, ph, ahead, pick)
+        _close(got[at], want[at], tol[at])
+        _close(lse[at], wl[at], lt[at])
+        assert (got[behind] == 0).all() and np.isfinite(got).all()
+
+
+@gpu
 @pytest.mark.parametrize("rows,batch,kvh,hd,most", [(1, 3, 2, 64, 2400), (6, 20, 3, 128, 1500),
                                                     (30, 2, 2, 64, 2400)])
 def test_rows_that_are_not_there(backend, pkg, rows, batch, kvh, hd, most):

@@ -155,6 +155,21 @@ def test_matches_the_rule(backend, pkg, batch, rows, n, temperature, one_hot):
 
 
 @gpu
+@pytest.mark.parametrize("batch,rows,n,temperature", [(2, 1, 1 << 20, 1.0), (1, 2, (1 << 20) - 1, 0.6),
+                                                      (3, 1, 65537, 1.0), (2, 1, 1 << 20, 0.0),
+                                                      (1, 1024, 33, 1.0), (300, 2, 70, 1.0)])
+def test_largest_sizes(backend, pkg, batch, rows, n, temperature):
+    rng = np.random.default_rng(n + batch)
+    target, draft, tokens, u = make(rng, batch, rows, n, near=0.3)
+    check(pkg, backend, target, draft, tokens, temperature, u, None)
+    # Draws near the end of the walk, and drafts that are all refused.
+    u[:, rows] = 1 - 2.0 ** -20
+    tokens[:] = (target[:, :rows].argmin(-1)).astype(np.uint32)
+    check(pkg, backend, target, draft, tokens, temperature, u, None)
+    check(pkg, backend, target, None, tokens, temperature, u, None)
+
+
+@gpu
 def test_accepts_all_and_none(backend, pkg):
     rng = np.random.default_rng(2)
     target, draft, tokens, u = make(rng, 6, 4, 3000, near=0.0)  # p == q: all accepted
