@@ -248,25 +248,19 @@ __device__ __forceinline__ uint32_t pair_f16(uint32_t a, uint32_t b) {
 // bits, lo the rest rounded to 11 (together within 2^-22, or 2^-25 below fp16's
 // normal range).
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-  // lo = x - hi in one instruction each (in C they become conversions and sums, three).
-  asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(hi), "v"(a));
-  asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-      : "+v"(lo)
-      : "v"(hi), "v"(b));
+  const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+  const h2 l = {(_Float16)fmaf((float)h[0], -1.f, a), (_Float16)fmaf((float)h[1], -1.f, b)};
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
 }
-
 // The same with lo times 2^11 (a, b at most 2^15), for weights: it keeps what lies below hi of
 // the smallest ones too.
 __device__ __forceinline__ void split2_up(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const float up = -2048.f;
-  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-  asm("v_fma_mixlo_f16 %0, %1, %3, %2 op_sel_hi:[1,0,0]"
-      : "=v"(lo)
-      : "v"(hi), "v"(a * 2048.f), "s"(up));
-  asm("v_fma_mixhi_f16 %0, %1, %3, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-      : "+v"(lo)
-      : "v"(hi), "v"(b * 2048.f), "s"(up));
+  const h2 h = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+  const h2 l = {(_Float16)fmaf((float)h[0], -2048.f, a * 2048.f),
+                (_Float16)fmaf((float)h[1], -2048.f, b * 2048.f)};
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
 }
 
 __device__ __forceinline__ int byte_s(uint32_t w, int i) { return (int)(int8_t)(w >> (8 * i)); }
