@@ -141,8 +141,7 @@ __device__ Step walk(double w, double base, double point, StepShared& sh) {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // 2^(n + f) from m = 1.5 2^52 + n and |f| <= 1/2: the polynomial that agrees
 // with 2^f in the ten Chebyshev points of [-1/2, 1/2] (within 4e-14 of it, and
-// 1 at 0), n put into the exponent field as an integer: so every
-// step is a full-rate f64 operation.
+// 1 at 0), times 2^n, n being m's low half as an integer.
 __device__ __forceinline__ double power2(double m, double f) {
   double p = 0x1.b6571de2f2351p-24;
   p = fma(p, f, 0x1.63ef969a64d3cp-20);
@@ -154,10 +153,7 @@ __device__ __forceinline__ double power2(double m, double f) {
   p = fma(p, f, 0x1.ebfbdff8149f2p-3);
   p = fma(p, f, 0x1.62e42fefa39f7p-1);
   p = fma(p, f, 1.0);
-  // (One instruction: in C the halves become a 64-bit sum of five.)
-  u32x2 u = __builtin_bit_cast(u32x2, p);
-  asm("v_lshl_add_u32 %0, %1, 20, %0" : "+v"(u.y) : "v"(__builtin_bit_cast(u32x2, m).x));
-  return __builtin_bit_cast(double, u);
+  return ldexp(p, (int)__builtin_bit_cast(u32x2, m).x);
 }
 // Weight 2^(c (l - max)) of a logit next to its row's (or part's) maximum; none
 // for a NaN, and for an infinity next to an infinite maximum.  (Weights below
