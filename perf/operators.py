@@ -16,7 +16,11 @@ and their exponents ([slots][kv_heads][cap], int8 as well), where ``row`` is
 32, and a value is code * 2^exponent.
 
 With ``own`` false the operators are computed in their plain form from the
-same buffers; with ``own`` true by the library's kernels.
+same buffers; with ``own`` true by the library's kernels, queued on the
+backend's stream, which neither waits for torch's nor is waited for by it: a
+state's first pass waits for the device, so that its inputs are there and
+nothing of torch's still uses the memory of its outputs; whoever reads a
+pass's outputs by torch, or drops a state, synchronises the device before.
 """
 
 import ctypes
@@ -430,6 +434,7 @@ def _own_pass(state):
     c, kind = state["case"], state["case"]["kind"]
     if "plan" not in state:
         state["plan"] = _plan(state)
+        torch.cuda.synchronize()
     p = state["plan"]
     out, b, r = p["out"], c["batch"], c["rows"]
     if kind == "verify":
