@@ -203,13 +203,17 @@ __global__ __launch_bounds__(256) void k_cache_read_q8(Q8Cache c, float* k, floa
 // row c of MFMA j.
 //
 // The exponents: a key's K scale multiplies its scores, its V scale its
-// weights.  Weights are kept at 2^(x - mt) 2^(ve - eb) with mt (per row) and
-// eb (per wave) such that the largest lies at 2^-4, whole powers of two; they
-// may grow to 2^15 (PACK: 61440) before mt and eb move and the accumulators are
-// rescaled (exactly), so most tiles neither join maxima across lanes nor
-// rescale.  lo is kept times 2^11 and meets V's codes times 2^-11 (PACK: its
-// column's results take the factor), so a weight loses what is below 2^-36 only, next to a
-// largest one of 2^-4.  With lo unscaled and levels at 2^6 the 32 rows of a
+// weights.  Sums add 2^(x - mt), products take w = 2^(x - mt) 2^(ve - ev), with
+// whole mt and ev of each row, from the keys that it sees, such that its largest w
+// lies at 2^-4; w may grow to 2^15 (PACK: 61440) before they move and the
+// accumulators are rescaled (exactly), so most tiles neither join maxima across
+// lanes nor rescale.  Mostly ev is 0: one 2^x serves both.  Where mt would then lie
+// 2^90 below the row's largest score, or a V scale of 2^90 meets 2^x below 32 bits'
+// normal range, the wave's rows are kept apart: mt by the scores alone, and w by a
+// 2^x of its own.  lo is kept times 2^11 and meets V's codes times 2^-11 (PACK: its
+// column's results take the factor), so a weight loses what is below 2^-36 (PACK,
+// which truncates lo: 2^-35) only, next to a largest one above 2^-5.  With lo
+// unscaled and levels at 2^6 the 32 rows of a
 // wave moved them so often that the barriers of blocks in LDS waited for one
 // wave or another: 69 us in place of 64 behind 8200 keys whose scales differ by 16.
 
@@ -268,7 +272,8 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4 exps_of(uint32_t w) {
   return i32x4{byte_s(w, 0), byte_s(w, 1), byte_s(w, 2), byte_s(w, 3)};
 }
-// K exponents from here on are applied next to q's (2^29 codes times more may leave f32).
+// K exponents from here on are applied next to q's (2^29 codes times more may leave f32), V's
+// of rows kept apart.
 constexpr int kBigExp = 90;
 
 // What one 32-key tile's lane loads.
@@ -507,17 +512,15 @@ __device__ __forceinline__ size_t row_id(const AttnQ8Args& a, const RowRef& r) {
 template <int ROW, int NT>
 struct RowsState {
   f32x4 acc[NT][ROW / 16];
-  float mt[NT], top_x[NT], top_w[NT], l[NT];
-  int eb;
-  bool fresh;
+  float mt[NT], ev[NT], l[NT];
+  bool fresh, apart;  // of the wave; ev is 0 unless apart
 
   __device__ __forceinline__ void init() {
-    eb = 0;
     fresh = true;
+    apart = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      mt[n] = 0.f;
-      top_x[n] = top_w[n] = -INFINITY;
+      mt[n] = ev[n] = 0.f;
       l[n] = 0.f;
 #pragma unroll
       for (int j = 0; j < ROW / 16; ++j) acc[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -528,7 +531,7 @@ struct RowsState {
 // One tile of 32 keys: kfrag(hh, s) and vfrag(j) give K's and V's A operands,
 // kexp(hh) and vexp(hh) the exponents of the lane's four keys of half hh (any number
 // in range behind the last key that any row sees), odd whether the tile has a NaN
-// row or a K exponent of kBigExp.  limit: keys a row sees; a tile past the least
+// row or an exponent of kBigExp.  limit: keys a row sees; a tile past the least
 // of them needs the mask.  k_used() is called once K's operands are spent.
 template <int ROW, int NT, bool PACK, class KF, class VF, class KE, class VE, class HK>
 __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*qh)[ROW / 32],
@@ -576,9 +579,11 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   int plain = -1;  // 0: K's exponents are applied already
   if (odd) {
     asm volatile("");
+    int high = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = kexp(i >> 2)[i & 3];
+      high = max(high, vexp(i >> 2)[i & 3]);
       const float f = e == kNanExp ? __int_as_float(0x7FC00000) : ldexpf(1.f, e);
 #pragma unroll
       for (int n = 0; n < NT; ++n) d[n][i >> 2][i & 3] *= f * qf[n];
@@ -586,6 +591,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
 #pragma unroll
     for (int n = 0; n < NT; ++n) qe[n] = 1.f;
     plain = 0;
+    if (__any(high >= kBigExp)) st.apart = true;
   }
   float w[NT][8], add[NT];
   auto weights = [&](auto masked) {
@@ -593,12 +599,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     for (int n = 0; n < NT; ++n) add[n] = 0.f;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
-      const i32x4 ke = kexp(hh) & plain;
-      i32x4 ve = vexp(hh);
-      if (st.eb != 0) {
-        asm volatile("");
-        ve -= st.eb;
-      }
+      const i32x4 ke = kexp(hh) & plain, ve = vexp(hh);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -608,6 +609,18 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
           if constexpr (decltype(masked)::value) p = sees(n, 4 * hh + r) ? p : 0.f;
           add[n] += p;
           w[n][4 * hh + r] = ldexpf(p, ve[r]);
+        }
+    }
+    if (st.apart) {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float x = ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] & plain);
+          const float p = __builtin_amdgcn_exp2f(fmaf(x, qe[n], -st.mt[n]) +
+                                                 ((float)vexp(i >> 2)[i & 3] - st.ev[n]));
+          w[n][i] = sees(n, i) ? p : 0.f;
         }
     }
   };
@@ -628,41 +641,47 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     }
   }
   if (__any(over)) {
-    // New levels: the largest x + ve of a row at 2^-4.  eb is 0 unless the
-    // values' scales are far from 1.
+    // New levels, of the keys that a row sees: with base the tile's largest score or the level
+    // before if that is higher, the largest w next to 2^base, in (2^(r - 5), 2^(r - 4)], at 2^-4.
     asm volatile("");
-    int high = -126;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) high = max(high, vexp(i >> 2)[i & 3]);
-    high = max(high, __shfl_xor(high, 16, 64));  // the columns' lanes hold the same keys
-    high = __builtin_amdgcn_readfirstlane(max(high, __shfl_xor(high, 32, 64)));
-    int eb1 = st.eb;
-    if (st.fresh ? high > 60 || high < -60 : st.eb == 0 ? high > 60 : high > st.eb) eb1 = high;
+    float base[NT], r[NT];
+    bool far = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      auto x = [&](int i) {
+        return ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] & plain) * qe[n];
+      };
       float mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] & plain) * qe[n];
-        const bool in = sees(n, i);
-        mx = fmaxf(mx, in ? x : -INFINITY);
-        mw = fmaxf(mw, in ? x + (float)vexp(i >> 2)[i & 3] : -INFINITY);
-      }
-      st.top_x[n] = fmaxf(st.top_x[n], ceilf(xor_max<32>(xor_max<16>(mx))));
-      st.top_w[n] = fmaxf(st.top_w[n], ceilf(xor_max<32>(xor_max<16>(mw))));
-      float m1 = fmaxf(st.top_w[n] - (float)eb1 - -4.f, st.top_x[n] - 90.f);  // (2^30 sums stay in f32)
-      if (m1 == -INFINITY) m1 = 0.f;  // no key yet
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sees(n, i) ? x(i) : -INFINITY);
+      base[n] = fmaxf(st.fresh ? -INFINITY : st.mt[n], ceilf(xor_max<32>(xor_max<16>(mx))));
+      if (base[n] == -INFINITY) base[n] = 0.f;  // no key yet
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        mw = fmaxf(mw, sees(n, i) ? (x(i) - base[n]) + (float)vexp(i >> 2)[i & 3] : -INFINITY);
+      r[n] = ceilf(xor_max<32>(xor_max<16>(mw))) + 4.f;
+      if (!st.fresh) r[n] = fmaxf(r[n], (st.mt[n] - base[n]) + st.ev[n]);
+      if (r[n] == -INFINITY) r[n] = 0.f;
+      // One level for both, base + r: 2^30 sums of up to 2^90 stay in f32, and next to a large
+      // score it may not be a 32-bit number.
+      far |= r[n] < -90.f || (base[n] + r[n]) - base[n] != r[n];
+    }
+    if (__any(far)) st.apart = true;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m1 = st.apart ? base[n] : base[n] + r[n], e1 = st.apart ? r[n] : 0.f;
       if (!st.fresh) {
-        st.l[n] *= __builtin_amdgcn_exp2f(st.mt[n] - m1);
-        const float keep = __builtin_amdgcn_exp2f(st.mt[n] - m1 + (float)(st.eb - eb1));
+        const float by = st.mt[n] - m1;
+        st.l[n] *= __builtin_amdgcn_exp2f(by);
+        const float keep = __builtin_amdgcn_exp2f(by + (st.ev[n] - e1));
 #pragma unroll
         for (int j = 0; j < DT; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) st.acc[n][j][r] *= keep;
+          for (int i = 0; i < 4; ++i) st.acc[n][j][i] *= keep;
       }
       st.mt[n] = m1;
+      st.ev[n] = e1;
     }
-    st.eb = eb1;
     st.fresh = false;
     weights(std::true_type{});
   }
@@ -877,7 +896,7 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       low = min(low, min(min(e0[r], e1[r]), min(f0[r], f1[r])));
-      high = max(high, max(e0[r], e1[r]));
+      high = max(high, max(max(e0[r], e1[r]), max(f0[r], f1[r])));
     }
     const bool more = t + 2 * WAVES < t1;
     tile_step<ROW, 1, PACK>(
@@ -922,10 +941,10 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
         if constexpr (PACK) o[i] = fmaf(dpp_f32<0x128>(o[i]), 0x1p-11f, o[i]);
         o[i] *= inv;
       }
-      if (st.eb != 0) {
+      if (st.apart) {
         asm volatile("");
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], st.eb);
+        for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], (int)st.ev[0]);
       }
       if (mine && ref.live) *reinterpret_cast<f32x4*>(&so[wave][c][(4 * g + r) * DT + j]) = o;
     }
@@ -1111,7 +1130,7 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
       const int ek = re_in ? re[0] : 0, ev = re_in ? re[1] : 0;
       exps[half][0][lane] = ek;
       exps[half][1][lane] = ev;
-      const uint64_t odd = __ballot(ek == kNanExp || ev == kNanExp || ek >= kBigExp);
+      const uint64_t odd = __ballot(min(ek, ev) == kNanExp || max(ek, ev) >= kBigExp);
       if (lane < 2) odds[half][lane] = (uint32_t)(odd >> (32 * lane));
     }
   };
@@ -1208,12 +1227,12 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     const float inv = total[n] == 0.f ? 0.f : 1.f / total[n];
 #pragma unroll
     for (int j = 0; j < DT; ++j) st.acc[n][j] *= inv;
-    if (st.eb != 0) {
+    if (st.apart) {
       asm volatile("");
 #pragma unroll
       for (int j = 0; j < DT; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) st.acc[n][j][r] = ldexpf(st.acc[n][j][r], st.eb);
+        for (int r = 0; r < 4; ++r) st.acc[n][j][r] = ldexpf(st.acc[n][j][r], (int)st.ev[n]);
     }
   }
   const int row = rw * 32 + c;  // + 16 for the rows of kw = 1

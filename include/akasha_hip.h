@@ -336,9 +336,10 @@ akh_status akh_attn_q8_workspace(const akh_attn_q8* shape, const akh_q8_cache* c
  * counts[b] get zeros and -infinity, and what q holds in them is not looked
  * at.  Products in two fp16 terms (22 bits) of q and of the softmax weights
  * with the exact codes, sums in f32: the accuracy of f32 arithmetic on the
- * cache's values.  What a key adds is kept to 2^-22 of itself and 2^-32 of the
- * most that a key adds to the row.  NaN and infinities in q and NaN rows of the cache make the
- * heads that use them NaN. */
+ * cache's values.  What a key adds to a row is kept to 2^-21 of itself and 2^-29 of the
+ * most that a key adds to it, whatever the scales of the values and of keys that it does not
+ * see; weights below 2^-126 of the row's largest may be lost.  NaN and infinities in q
+ * and NaN rows of the cache make the heads that use them NaN. */
 akh_status akh_attn_cached_q8(akh_backend* be, const float* q, akh_q8_cache cache, float* out,
                               float* lse, akh_attn_q8 shape, const uint32_t* pos,
                               const uint32_t* counts, void* workspace, size_t workspace_bytes);
