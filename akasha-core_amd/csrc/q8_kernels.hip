@@ -504,6 +504,12 @@ struct RawQ {
 struct PartMl {
   float m, l;
 };
+// A part's sum next to level `top`.  Levels are whole numbers, and those of parts whose V scales
+// are far apart may differ by 2^184 where their sums do by the inverse: as a factor, 2^(m - top)
+// could leave f32.
+__device__ __forceinline__ float part_sum(const PartMl& p, float top) {
+  return p.l == 0.f ? 0.f : ldexpf(p.l, (int)fmaxf(p.m - top, -1000.f));
+}
 __device__ __forceinline__ size_t row_id(const AttnQ8Args& a, const RowRef& r) {
   return r.bt * a.heads + r.head;
 }
@@ -973,11 +979,11 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
 #pragma unroll
     for (int i = 0; i < NP; ++i) m = fmaxf(m, pre[i].m);
     m = group_max<L>(m);
-    const float f = y.l == 0.f ? 0.f : y.l * __builtin_amdgcn_exp2f(y.m - m);
+    const float f = part_sum(y, m);
     float sum = f, z[NP > 0 ? NP : 1];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      z[i] = pre[i].l == 0.f ? 0.f : pre[i].l * __builtin_amdgcn_exp2f(pre[i].m - m);
+      z[i] = part_sum(pre[i], m);
       sum += z[i];
     }
     sum = group_sum<L>(sum);
@@ -1261,12 +1267,9 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     const PartMl y = sml[row + r16];
     float top = fmaxf(mm, y.m);
     for (uint32_t e = 0; e < extra && x.live; ++e) top = fmaxf(top, ml[part + e].m);
-    auto weight_of = [&](const PartMl& z, float top) {
-      return z.l == 0.f ? 0.f : z.l * __builtin_amdgcn_exp2f(z.m - top);
-    };
-    const float f0 = weight_of({mm, ll}, top), f1 = weight_of(y, top);
+    const float f0 = part_sum({mm, ll}, top), f1 = part_sum(y, top);
     float sum = f0 + f1;
-    for (uint32_t e = 0; e < extra && x.live; ++e) sum += weight_of(ml[part + e], top);
+    for (uint32_t e = 0; e < extra && x.live; ++e) sum += part_sum(ml[part + e], top);
     const float inv = x.live && sum != 0.f ? 1.f / sum : 0.f;
     float* mine = so + (size_t)(row + r16) * RS + 4 * g * DT;
 #pragma unroll
@@ -1292,7 +1295,7 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
         const float t = __shfl(top, r, 64), n = __shfl(inv, r, 64);
         if (lives >> r & 1)
           for (uint32_t e = 0; e < extra; ++e)
-            o += weight_of(ml[p + e], t) * n * *reinterpret_cast<const f32x4*>(po + (p + e) * ROW + col);
+            o += part_sum(ml[p + e], t) * n * *reinterpret_cast<const f32x4*>(po + (p + e) * ROW + col);
       }
       if (!(lives >> r & 1)) o = f32x4{0.f, 0.f, 0.f, 0.f};
       if (flags >> r & 1) {
@@ -1342,8 +1345,7 @@ __global__ __launch_bounds__(256) void k_attn_q8_join(AttnQ8Args a, AttnQ8Plan p
     m = wave_max(fmaxf(y[0].m, y[1].m));
     float f[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      f[i] = y[i].l == 0.f ? 0.f : y[i].l * __builtin_amdgcn_exp2f(y[i].m - m);
+    for (int i = 0; i < 2; ++i) f[i] = part_sum(y[i], m);
     total = wave_sum(f[0] + f[1]);
     const float inv = total == 0.f ? 0.f : 1.f / total;
     f[0] *= inv;

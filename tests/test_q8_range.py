@@ -126,3 +126,47 @@ def test_scores_of_2_to_the_30(backend, pkg, rows, heads, kvh, hd, n, size):
     # A weight of one: its two terms, the sum's reciprocal and products with it, in 32 bits.
     _close(got[0], np.broadcast_to(want, got[0].shape), np.abs(want) * 2.0 ** -19)
     _close(lse[0], np.full((rows, heads), held.k[0, 0, at, 0]), 2.0 ** 30 * 2.0 ** -21)
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd,n", SHAPES)
+@pytest.mark.parametrize("own,pre", [(58, -100), (-100, 58), (85, -85), (-85, 85), (115, -115),
+                                     (-120, 0), (0, 119)])
+def test_parts_whose_values_are_far_apart(backend, pkg, rows, heads, kvh, hd, n, own, pre):
+    # Own rows and prefix weigh the same, and one key of either, which weighs nothing, has a
+    # scale of its own.
+    rng = np.random.default_rng(rows * heads + hd + 200 + own)
+    batch, scale, ahead, most = 2, 0.125, 200, min(n, 333)
+    parts = []
+    for slots, length, exp in ((batch, most, own), (1, ahead, pre)):
+        bias, size = np.zeros((slots, length)), np.full((slots, length), float(exp))
+        bias[:, 5], size[:, 5] = -200, -10
+        k = _biased(rng, slots, length, kvh, hd, bias, scale).astype(np.float32)
+        v = rng.standard_normal(k.shape) * np.exp2(size)[..., None, None]
+        parts.append(_cache(pkg, backend, k, v.astype(np.float32)))
+    (cache, held), (prefix, pheld) = parts
+    q = _queries(rng, batch, rows, heads, hd)
+    pos = [most - rows, most - rows - 40]
+    got, lse = _attend(pkg, backend, q, cache, pos, None, scale, prefix, ahead)
+    want, wl, tol, lt = fine(q, held, pos, [rows] * batch, scale, pheld, ahead)
+    _close(got, want, tol)
+    _close(lse, wl, lt)
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd,n", SHAPES)
+@pytest.mark.parametrize("most", [70, 85, 115])
+def test_values_that_grow_along_the_keys(backend, pkg, rows, heads, kvh, hd, n, most):
+    # Waves, halves and splits of the keys meet scales of their own; growing and falling.
+    rng = np.random.default_rng(rows * heads + hd + n + most)
+    batch, scale = 2, 0.125
+    size = np.linspace(-most, most, n)
+    k = _biased(rng, batch, n, kvh, hd, 0, scale).astype(np.float32)
+    v = rng.standard_normal(k.shape) * np.exp2(np.stack([size, size[::-1]]))[..., None, None]
+    cache, held = _cache(pkg, backend, k, v.astype(np.float32))
+    q = _queries(rng, batch, rows, heads, hd)
+    pos = [n - rows, n - rows - 40]
+    got, lse = _attend(pkg, backend, q, cache, pos, None, scale)
+    want, wl, tol, lt = fine(q, held, pos, [rows] * batch, scale)
+    _close(got, want, tol)
+    _close(lse, wl, lt)
