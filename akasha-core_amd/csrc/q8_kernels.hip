@@ -617,6 +617,8 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
           w[n][4 * hh + r] = ldexpf(p, ve[r]);
         }
     }
+  };
+  auto weights_apart = [&]() {
     if (st.apart) {
       asm volatile("");
 #pragma unroll
@@ -638,6 +640,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     } else {
       weights(std::false_type{});
     }
+    weights_apart();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float big = 0.f;
@@ -690,6 +693,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     }
     st.fresh = false;
     weights(std::true_type{});
+    weights_apart();
   }
   if (odd) {  // a row that sees a NaN row of V becomes NaN (K's made its scores NaN)
     asm volatile("");
