@@ -575,7 +575,8 @@ struct AttnQ8Args {
   float scale;
   void* ws;
   // Set by the launch:
-  float scale_log2;     // scale * log2(e)
+  float scale_mant;     // scale * log2(e), of [1/2, 1] times 2^scale_exp
+  int scale_exp;
   bool q_vec, out_vec;  // rows of q and out can be read as float4
 };
 // How an attention call is dealt to blocks, from its sizes alone.

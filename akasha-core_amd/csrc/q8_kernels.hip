@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -275,6 +276,12 @@ __device__ __forceinline__ i32x4 exps_of(uint32_t w) {
 // K exponents from here on are applied next to q's (2^29 codes times more may leave f32), V's
 // of rows kept apart.
 constexpr int kBigExp = 90;
+// In the place of q's exponent for rows that are not there: they weigh every key alike, so that
+// their scores move no levels.
+constexpr int kNoRow = -1000;
+__device__ __forceinline__ bool outside_f32(int qx) {
+  return qx != kNoRow && (qx < -126 || qx > 127);
+}
 
 // What one 32-key tile's lane loads.
 template <int ROW>
@@ -474,19 +481,27 @@ struct RawQ {
   }
 
   // As B operands, hi and lo, times scale log2(e) 2^-e with a largest magnitude
-  // in [2^13, 2^14] or next to it; returns 2^e.  A NaN or an infinity makes one
+  // in [2^13, 2^14]; returns e.  The scale comes as mantissa and exponent, so that
+  // its product with q does not leave f32.  A NaN or an infinity makes one
   // of the terms NaN (inf - inf), and with it the row's scores.
-  __device__ __forceinline__ float operands(const AttnQ8Args& a, f16x8* hi, f16x8* lo) {
+  __device__ __forceinline__ int operands(const AttnQ8Args& a, f16x8* hi, f16x8* lo) {
     float top = 0.f;
 #pragma unroll
     for (int s = 0; s < ROW / 32; ++s)
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[s][i]));
-    top = xor_max<32>(xor_max<16>(top)) * fabsf(a.scale_log2);
-    // top = 1.m 2^(E - 127); times 2^(140 - E) it is 1.m 2^13 (E at least 40, so
-    // that the factor is a normal number; smaller rows keep small terms).
-    const int E = max(40, (int)(__float_as_uint(top) >> 23));
-    const float f = ldexpf(a.scale_log2, 140 - E);
+    top = xor_max<32>(xor_max<16>(top));
+    const float m = __builtin_amdgcn_frexp_mantf(top) * fabsf(a.scale_mant);
+    const int up = 14 - __builtin_amdgcn_frexp_expf(top) + (m < 0.5f);
+    const int first = up > 126 ? up - 126 : 0;  // of the smallest rows, whose factor leaves f32
+    if (__any(first != 0)) {
+      asm volatile("");
+#pragma unroll
+      for (int s = 0; s < ROW / 32; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[s][i] = ldexpf(x[s][i], first);
+    }
+    const float f = ldexpf(a.scale_mant, up - first);
 #pragma unroll
     for (int s = 0; s < ROW / 32; ++s) {
       uint32_t h[4], l[4];
@@ -495,7 +510,7 @@ struct RawQ {
       hi[s] = f16x8_of(make_uint4(h[0], h[1], h[2], h[3]));
       lo[s] = f16x8_of(make_uint4(l[0], l[1], l[2], l[3]));
     }
-    return ldexpf(1.f, E - 140);
+    return a.scale_exp - up;
   }
 };
 
@@ -537,11 +552,13 @@ struct RowsState {
 // One tile of 32 keys: kfrag(hh, s) and vfrag(j) give K's and V's A operands,
 // kexp(hh) and vexp(hh) the exponents of the lane's four keys of half hh (any number
 // in range behind the last key that any row sees), odd whether the tile has a NaN
-// row or an exponent of kBigExp.  limit: keys a row sees; a tile past the least
+// row or an exponent of kBigExp, or a row a q exponent outside f32.  qx(n): exponents of q's
+// operands, kNoRow for rows that are not there.  limit: keys a row sees; a tile past the least
 // of them needs the mask.  k_used() is called once K's operands are spent.
-template <int ROW, int NT, bool PACK, class KF, class VF, class KE, class VE, class HK>
+template <int ROW, int NT, bool PACK, class QX, class KF, class VF, class KE, class VE,
+          class HK>
 __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*qh)[ROW / 32],
-                                          const f16x8 (*ql)[ROW / 32], const float* qf,
+                                          const f16x8 (*ql)[ROW / 32], QX qx,
                                           const uint32_t* limit, uint32_t least, uint32_t tile,
                                           int g, int c, bool odd, KF kfrag, VF vfrag, KE kexp,
                                           VE vexp, HK k_used) {
@@ -581,7 +598,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   auto sees = [&](int n, int i) { return key0 + (i & 3) + (i >> 2) * 16 < limit[n]; };
   float qe[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) qe[n] = qf[n];
+  for (int n = 0; n < NT; ++n) qe[n] = ldexpf(1.f, qx(n));
   int plain = -1;  // 0: K's exponents are applied already
   if (odd) {
     asm volatile("");
@@ -590,9 +607,10 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     for (int i = 0; i < 8; ++i) {
       const int e = kexp(i >> 2)[i & 3];
       high = max(high, vexp(i >> 2)[i & 3]);
-      const float f = e == kNanExp ? __int_as_float(0x7FC00000) : ldexpf(1.f, e);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) d[n][i >> 2][i & 3] *= f * qf[n];
+      for (int n = 0; n < NT; ++n)
+        d[n][i >> 2][i & 3] = e == kNanExp ? __int_as_float(0x7FC00000)
+                                           : ldexpf(d[n][i >> 2][i & 3], e + qx(n));
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) qe[n] = 1.f;
@@ -848,14 +866,14 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
   }
   // Wave 0 makes the rows' operands for all.
   __shared__ uint4 sq[PACK ? 1 : 2][KS][64];
-  __shared__ float sqf[16];
+  __shared__ int sqx[16];
   const RowRef ref = job.row(a, row0 + (PACK ? c & 7 : c));
   if (wave == 0) {
     RawQ<ROW> raw;
     raw.load(a, ref, g);
     f16x8 hi[KS], lo[KS];
-    const float f = raw.operands(a, hi, lo);
-    if (g == 0) sqf[c] = f;
+    const int qe = raw.operands(a, hi, lo);
+    if (g == 0) sqx[c] = qe;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       sq[0][s][lane] = __builtin_bit_cast(uint4, PACK && c >= 8 ? lo[s] : hi[s]);
@@ -884,8 +902,8 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     qh[0][s] = f16x8_of(sq[0][s][lane]);
     if constexpr (!PACK) ql[0][s] = f16x8_of(sq[1][s][lane]);
   }
-  // Rows that are not there weigh every key alike, so that their scores move no levels.
-  const float qf = ref.live ? sqf[c] : 0.f;
+  const int qx = ref.live ? sqx[c] : kNoRow;
+  const bool far = __any(outside_f32(qx));
   RowsState<ROW, 1> st;
   st.init();
   auto step = [&](Tile<ROW>& tile) {
@@ -910,7 +928,8 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
     }
     const bool more = t + 2 * WAVES < t1;
     tile_step<ROW, 1, PACK>(
-        st, qh, ql, &qf, &ref.limit, least, t, g, c, __any(low == kNanExp || high >= kBigExp),
+        st, qh, ql, [&](int) { return qx; }, &ref.limit, least, t, g, c,
+        far || __any(low == kNanExp || high >= kBigExp),
         [&](int hh, int s) {
           const uint4 w = tile.k[hh][s >> 1];
           return (s & 1) ? codes8_f16(w.z, w.w) : codes8_f16(w.x, w.y);
@@ -1059,7 +1078,7 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   __shared__ uint4 smem[kBuffers > kJoin ? kBuffers : kJoin];
   __shared__ __attribute__((aligned(16))) int exps[2][2][64];  // a stage's exponents, K's and V's
   __shared__ uint32_t odds[2][2];  // whether its tiles are odd
-  __shared__ float sqf[32 * RW];
+  __shared__ int sqx[32 * RW];
   static_assert((size_t)W * KS * 2 * 64 <= kBuffers, "the rows' operands fit the buffers");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1176,8 +1195,8 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     RawQ<ROW> raw;
     raw.from_lds(own, RS, g, c);
     f16x8 hi[KS], lo[KS];
-    const float f = raw.operands(a, hi, lo);
-    if (g == 0) sqf[wave * 16 + c] = f;
+    const int qe = raw.operands(a, hi, lo);
+    if (g == 0) sqx[wave * 16 + c] = x.live ? qe : kNoRow;
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -1188,13 +1207,15 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
   RowRef ref[NT];
   uint32_t limit[NT];
   f16x8 qh[NT][KS], ql[NT][KS];
-  float qf[NT];
+  bool far = false;
+  int qx[NT];
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     ref[n] = job.row(a, row0 + n * 16 + c);
     limit[n] = ref[n].limit;
-    qf[n] = ref[n].live ? sqf[rw * 32 + n * 16 + c] : 0.f;  // as in k_attn_q8
+    qx[n] = sqx[rw * 32 + n * 16 + c];
+    far |= __any(outside_f32(qx[n]));
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qh[n][s] = f16x8_of(smem[(((rw * 2 + n) * KS + s) * 2) * 64 + lane]);
@@ -1213,8 +1234,8 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
       const uint4* f = smem + ((size_t)half * 2 + kw) * FRAGS * 64 + lane;
       const int* e = &exps[half][0][32 * kw + 4 * g];
       tile_step<ROW, NT, false>(
-          st, qh, ql, qf, limit, least, t + kw, g, c,
-          __builtin_amdgcn_readfirstlane(odds[half][kw]) != 0,
+          st, qh, ql, [&](int n) { return qx[n]; }, limit, least, t + kw, g, c,
+          far || __builtin_amdgcn_readfirstlane(odds[half][kw]) != 0,
           [&](int hh, int s) { return f16x8_of(f[(hh * KS + s) * 64]); },
           [&](int j) { return f16x8_of(f[(2 * KS + j) * 64]); },
           [&](int hh) { return *reinterpret_cast<const i32x4*>(e + 16 * hh); },
@@ -1554,7 +1575,7 @@ size_t attn_q8_workspace_bytes(const AttnQ8Args& a, bool prefix) {
 
 hipError_t launch_attn_q8(AttnQ8Args a, hipStream_t s) {
   const AttnQ8Plan p = attn_q8_plan(a, a.prefix_len != nullptr);
-  a.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+  a.scale_mant = (float)std::frexp((double)a.scale * 1.4426950408889634, &a.scale_exp);
   a.q_vec = vec4(a.q, a.q_stride, a.c.head_dim);
   a.out_vec = vec4(a.out, a.out_stride, a.c.head_dim);
   return a.c.row == 128 ? launch_attn<128>(a, p, s) : launch_attn<64>(a, p, s);

@@ -170,3 +170,46 @@ def test_values_that_grow_along_the_keys(backend, pkg, rows, heads, kvh, hd, n, 
     want, wl, tol, lt = fine(q, held, pos, [rows] * batch, scale)
     _close(got, want, tol)
     _close(lse, wl, lt)
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd,n", SHAPES)
+def test_queries_of_any_scale(backend, pkg, rows, heads, kvh, hd, n):
+    # q and K scaled against each other, from subnormal queries to those next to 2^127; among a
+    # sequence's rows some of ordinary scores and some of none.
+    rng = np.random.default_rng(rows * heads + hd + n)
+    by = [-104, -107, -114, -118, -124, 60, 100, 117]
+    batch, n, scale = len(by), min(n, 333), 0.125
+    k = rng.standard_normal((batch, n, kvh, hd)) * np.exp2(-np.float64(by))[:, None, None, None]
+    v = rng.standard_normal(k.shape)
+    q = rng.standard_normal((batch, rows, heads, hd)) * np.exp2(np.float64(by))[:, None, None, None]
+    q[:5, 1::3] *= 2.0 ** -20
+    with np.errstate(under="ignore"):
+        k, v, q = (x.astype(np.float32) for x in (k, v, q))
+    cache, held = _cache(pkg, backend, k, v)
+    pos = [n - rows] * batch
+    got, lse = _attend(pkg, backend, q, cache, pos, None, scale)
+    want, wl, tol, lt = fine(q, held, pos, [rows] * batch, scale)
+    _close(got, want, tol)
+    _close(lse, wl, lt)
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd,n", SHAPES)
+@pytest.mark.parametrize("scale,by_q,by_k", [(2.0 ** 127, -120, -10), (3e38, -60, -70),
+                                             (2.0 ** 100, -126, 20), (2.0 ** -140, 60, 78),
+                                             (2.0 ** -126, 120, 4), (-2.0 ** 90, 30, -122),
+                                             (0.0, 0, 0)])
+def test_any_scale(backend, pkg, rows, heads, kvh, hd, n, scale, by_q, by_k):
+    rng = np.random.default_rng(rows * heads + hd + n)
+    batch, n = 2, min(n, 333)
+    scale = float(np.float32(scale))
+    k = (rng.standard_normal((batch, n, kvh, hd)) * 2.0 ** by_k).astype(np.float32)
+    v = rng.standard_normal(k.shape).astype(np.float32)
+    q = (rng.standard_normal((batch, rows, heads, hd)) * 2.0 ** by_q).astype(np.float32)
+    cache, held = _cache(pkg, backend, k, v)
+    pos = [n - rows, n - rows - 70]
+    got, lse = _attend(pkg, backend, q, cache, pos, None, scale)
+    want, wl, tol, lt = fine(q, held, pos, [rows] * batch, scale)
+    _close(got, want, tol)
+    _close(lse, wl, lt)
