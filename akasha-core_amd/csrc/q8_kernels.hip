@@ -494,7 +494,7 @@ struct RawQ {
     const float m = __builtin_amdgcn_frexp_mantf(top) * fabsf(a.scale_mant);
     const int up = 14 - __builtin_amdgcn_frexp_expf(top) + (m < 0.5f);
     const int first = up > 126 ? up - 126 : 0;  // of the smallest rows, whose factor leaves f32
-    if (__any(first != 0)) {
+    if (__builtin_expect(__any(first != 0), 0)) {
       asm volatile("");
 #pragma unroll
       for (int s = 0; s < ROW / 32; ++s)
@@ -586,7 +586,8 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
   }
   k_used();
   // The rare cases are branches of their own that patch what the common path
-  // made (the empty asm keeps them branches).
+  // made (the empty asm keeps them branches, the expectation out of its way: 2 to 5% of
+  // a call).
   const uint32_t key0 = tile * 32 + 4 * g;  // + r, and + 16 + r in the second half
   if constexpr (PACK) {
 #pragma unroll
@@ -600,7 +601,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
 #pragma unroll
   for (int n = 0; n < NT; ++n) qe[n] = ldexpf(1.f, qx(n));
   int plain = -1;  // 0: K's exponents are applied already
-  if (odd) {
+  if (__builtin_expect(odd, 0)) {
     asm volatile("");
     int high = 0;
 #pragma unroll
@@ -615,7 +616,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
 #pragma unroll
     for (int n = 0; n < NT; ++n) qe[n] = 1.f;
     plain = 0;
-    if (__any(high >= kBigExp)) st.apart = true;
+    if (__builtin_expect(__any(high >= kBigExp), 0)) st.apart = true;
   }
   float w[NT][8], add[NT];
   auto weights = [&](auto masked) {
@@ -637,7 +638,7 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     }
   };
   auto weights_apart = [&]() {
-    if (st.apart) {
+    if (__builtin_expect(st.apart, 0)) {
       asm volatile("");
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -675,25 +676,27 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     bool far = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      auto x = [&](int i) {
-        return ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] & plain) * qe[n];
-      };
-      float mx = -INFINITY, mw = -INFINITY;
+      float x[8], mx = -INFINITY, mw = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sees(n, i) ? x(i) : -INFINITY);
+      for (int i = 0; i < 8; ++i) {
+        x[i] = ldexpf(d[n][i >> 2][i & 3], kexp(i >> 2)[i & 3] & plain) * qe[n];
+        x[i] = sees(n, i) ? x[i] : -INFINITY;
+        mx = fmaxf(mx, x[i]);
+      }
       base[n] = fmaxf(st.fresh ? -INFINITY : st.mt[n], ceilf(xor_max<32>(xor_max<16>(mx))));
       if (base[n] == -INFINITY) base[n] = 0.f;  // no key yet
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        mw = fmaxf(mw, sees(n, i) ? (x(i) - base[n]) + (float)vexp(i >> 2)[i & 3] : -INFINITY);
+        mw = fmaxf(mw, (x[i] - base[n]) + (float)vexp(i >> 2)[i & 3]);
       r[n] = ceilf(xor_max<32>(xor_max<16>(mw))) + 4.f;
       if (!st.fresh) r[n] = fmaxf(r[n], (st.mt[n] - base[n]) + st.ev[n]);
       if (r[n] == -INFINITY) r[n] = 0.f;
       // One level for both, base + r: 2^30 sums of up to 2^90 stay in f32, and next to a large
       // score it may not be a 32-bit number.
       far |= r[n] < -90.f || (base[n] + r[n]) - base[n] != r[n];
+      __builtin_amdgcn_sched_barrier(0);  // a row's numbers at a time: registers
     }
-    if (__any(far)) st.apart = true;
+    if (__builtin_expect(__any(far), 0)) st.apart = true;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float m1 = st.apart ? base[n] : base[n] + r[n], e1 = st.apart ? r[n] : 0.f;
@@ -713,7 +716,8 @@ __device__ __forceinline__ void tile_step(RowsState<ROW, NT>& st, const f16x8 (*
     weights(std::true_type{});
     weights_apart();
   }
-  if (odd) {  // a row that sees a NaN row of V becomes NaN (K's made its scores NaN)
+  if (__builtin_expect(odd, 0)) {
+    // A row that sees a NaN row of V becomes NaN (K's made its scores NaN).
     asm volatile("");
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -970,7 +974,7 @@ __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ
         if constexpr (PACK) o[i] = fmaf(dpp_f32<0x128>(o[i]), 0x1p-11f, o[i]);
         o[i] *= inv;
       }
-      if (st.apart) {
+      if (__builtin_expect(st.apart, 0)) {
         asm volatile("");
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = ldexpf(o[i], (int)st.ev[0]);
@@ -1258,7 +1262,7 @@ __global__ __launch_bounds__(128 * RW, 2) void k_attn_q8_rows(AttnQ8Args a, Attn
     const float inv = total[n] == 0.f ? 0.f : 1.f / total[n];
 #pragma unroll
     for (int j = 0; j < DT; ++j) st.acc[n][j] *= inv;
-    if (st.apart) {
+    if (__builtin_expect(st.apart, 0)) {
       asm volatile("");
 #pragma unroll
       for (int j = 0; j < DT; ++j)
