@@ -1524,8 +1524,12 @@ AttnQ8Plan attn_q8_plan(const AttnQ8Args& a, bool prefix) {
   p.own_waves = d.waves;
   // Caches that the 256 MB behind the L2s will not hold until they are read
   // again: 64 sequences x 16 heads of 128, us with and without streaming:
-  // 256 rows (68 MB) 17.2 and 15.9, 512 27.9 and 30.2, 2048 88.3 and 96.7.
-  p.stream = (uint64_t)a.batch * a.c.kv_heads * a.max_len * 2 * a.c.row > (96ull << 20);
+  // 256 rows (68 MB) 17.2 and 15.9, 512 27.9 and 30.2, 2048 88.3 and 96.7.  Not with several
+  // groups of query rows, which read the same codes by way of one L2: 64 x 20 rows over 2048 keys
+  // of 16 heads of 128 (2 groups) 179 and 157, 1 x 9 rows of 16 heads over 120000 keys of 4 heads of
+  // 128 (3 groups) 62.2 and 56.3, 64 x 24 rows over 2048 keys of 12 heads of 64 (2) 72.6 and 70.2.
+  p.stream = p.own_groups == 1 && (uint64_t)a.batch * a.c.kv_heads *
+                                      a.max_len * 2 * a.c.row > (96ull << 20);
   if (prefix) {  // its parts are joined with the own rows' in any case
     const Deal e = deal(a.c.kv_heads, all, div_up(a.pre.max_rows, 32), a.c.row, ids, true);
     p.prefix_rt = e.rt;

@@ -1,6 +1,6 @@
-"""Attention over 8-bit caches larger than the machine's own caches, whose codes are read past them:
-the blocks of 8 packed rows with two waves and those of 16 rows, at both row sizes, with one split
-of the keys and with several, against 64 bits."""
+"""Attention over 8-bit caches larger than the machine's own caches, whose codes are read past them
+unless several groups of query rows share them: the blocks of 8 packed rows with two waves and
+those of 16 rows, at both row sizes, with one split of the keys and with several, against 64 bits."""
 
 import numpy as np
 import pytest
