@@ -871,10 +871,10 @@ extern "C" akh_status akh_verify_drafts(akh_backend* be, const float* target, co
   CHECK_ARG(!isnan(temperature), "akh_verify_drafts: temperature is NaN");
   CHECK_ARG(temperature <= 0.0f || uniforms,
             "akh_verify_drafts: sampling (temperature > 0) needs uniforms");
+  if (!batch) return AKH_OK;
   CHECK_ARG(workspace && aligned16(workspace) && workspace_bytes >= need,
             "akh_verify_drafts: workspace missing, unaligned or smaller than "
             "akh_verify_drafts_workspace");
-  if (!batch) return AKH_OK;
   VerifyArgs a{};
   a.target = target;
   a.draft = temperature > 0.0f ? draft : nullptr;

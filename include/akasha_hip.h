@@ -272,7 +272,7 @@ akh_status akh_sample_rows_noalloc(akh_backend* be, const float* logits, uint32_
  * pos, counts and prefix_len are device arrays read when the kernels run, so
  * a captured graph follows them as it follows metas.  Every call is queued on
  * the backend's stream and allocates nothing.  Work for zero sequences or
- * rows is AKH_OK and does nothing.  A call of more work than one grid of 2^24 - 1
+ * rows is AKH_OK and does nothing (a sequence without drafts still gets its one token).  A call of more work than one grid of 2^24 - 1
  * blocks holds is refused (AKH_E_INVALID): attention of 2^24 query rows times
  * heads, cache rows of that many times 16 heads (8 above head_dim 64) by four
  * rows, drafts of that many logit rows times 4096 ids.  Buffers that a call writes

@@ -303,3 +303,13 @@ def test_refusals(pkg):
     assert call(batch=0) == 0
     with pytest.raises(h.InvalidArgument):
         h.verify_drafts_workspace(1, 1, 0)
+
+
+def test_no_sequences_need_no_workspace(pkg):
+    h = pkg.hip
+    mem = (C.c_char * 8192)()  # zeroed memory in a backend's place: nothing of it is used
+    be, x = C.cast(mem, C.c_void_p), C.c_void_p(1 << 21)
+    assert h.verify_drafts_workspace(0, 3, 100) == 0
+    for temperature in (0.0, 1.0):
+        assert h.load().akh_verify_drafts(be, x, x, x, 0, 3, 100, temperature, None, x, x, x, None,
+                                          None, 0) == 0
