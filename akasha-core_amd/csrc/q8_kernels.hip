@@ -818,9 +818,10 @@ __device__ __forceinline__ void store_out(const AttnQ8Args& a, uint64_t at, uint
 // 4 heads (42 splits each) take 52 us and 5.5 for the join.  32 sequences over
 // up to 511 keys of 12 heads of 64 take 6 us with warm caches and 10 without: the launch, three
 // memory latencies (lengths, codes, output) and 0.85 us a tile, of which
-// there are four in a row a wave.  Blocks of 8 waves, and 4 waves a SIMD at
-// 128 registers, were slower; so was loading a wave's second tile too before the
-// lengths are known (10.6 -> 11.1).
+// there are four in a row a wave.  Blocks of 8 waves take 12.6 us there in place of 10.1 (their
+// registers leave room for one on a CU), but 6.9 in place of 7.4 where blocks are few (one sequence of 301
+// keys); 4 waves a SIMD at 128 registers spilled, and loading a wave's second tile too before the
+// lengths are known was slower (10.6 -> 11.1).
 template <int ROW, bool PACK, int WAVES, bool SHARED, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES, ROW == 64 ? 3 : 2) void k_attn_q8(AttnQ8Args a, AttnQ8Plan pl) {
   constexpr int KS = ROW / 32;       // MFMA steps of a score
@@ -1466,9 +1467,9 @@ constexpr uint64_t kCus = 256;
 // memory and no other group reads them.  Blocks in LDS: 8 of their waves on a
 // CU, 7 or 8.5 us and 1.4 to 2.8 or 2.1 a stage of 64 keys.  Splits cost a join, and
 // their rows written and read.  Over 72 shapes drawn from 1 to 256 rows and 64 to
-// 30000 keys the choice's time is 1.2% above the fastest kind's of rows per block, 20% at
-// the worst; taking the largest block that the rows fill was up to 2 times it
-// (16 x 20 rows of 12 heads over 2, 400 keys: 17.8 us, here 8.5).
+// 30000 keys the choice's time is 0.9% above the fastest kind's of rows per block, 16% at
+// the worst (profiles/q8_plan_shapes.md); taking the largest block that the rows fill was up to
+// 2 times it (16 x 20 rows of 12 heads over 2, 400 keys: 17.8 us, here 8.5).
 struct Deal {
   uint32_t rt, groups, waves, splits;
 };

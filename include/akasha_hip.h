@@ -320,7 +320,7 @@ akh_status akh_cache_read_q8(akh_backend* be, akh_q8_cache cache, float* k, floa
  * query head h reads kv head h / (heads / kv_heads).  Row strides in floats,
  * at least heads * head_dim.  max_len: the longest pos[b] + rows expected; it
  * only shapes the launch and its workspace (0: the cache's max_rows), longer
- * sequences are attended to in full all the same. */
+ * sequences are attended to in full all the same.  A prefix's launch is shaped by its max_rows. */
 typedef struct {
   uint32_t batch, rows, heads, q_stride, out_stride;
   float scale;
